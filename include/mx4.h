@@ -421,6 +421,136 @@ mx4_status mx4_matmul_argmax(mx4_context *ctx, const void *x_dev, mx4_dtype x_ty
 mx4_status mx4_embed(mx4_context *ctx, const mx4_weight *w, const uint32_t *ids_dev, uint32_t count,
                      uint16_t *out_dev);
 
+/* ------------------------------------------------------------------------
+ * 3. A step over a paged key/value cache: what stands between the q|k|v and
+ *    the o projection (engine/src/lib.rs:337-450 with one cache a layer,
+ *    :324-335; here a cache in pages, several sequences in a call, and trees
+ *    of drafted tokens beside single tokens and prompts).
+ * ------------------------------------------------------------------------ */
+
+/* A key/value cache in pages, caller-owned device memory: k and v are bf16
+ * [layers][pages][kv_heads][page_tokens][head_dim], 16-byte aligned.
+ * layer_stride: elements from one layer to the next (0: packed). page_tokens is
+ * a power of two from 16 to 4096; head_dim is 64, 128 or 256. */
+typedef struct mx4_kv_cache {
+    uint16_t *k;
+    uint16_t *v;
+    uint64_t layer_stride;
+    uint32_t layers, pages, kv_heads, page_tokens, head_dim;
+} mx4_kv_cache;
+
+/* The tokens of one call and where they live. Sequence s has the call's tokens
+ * start[s] .. start[s + 1] - 1 (start[0] == 0, ascending, start[seqs] == tokens;
+ * a sequence may have none), which follow the cached[s] tokens it already has;
+ * its position p is row p % page_tokens of page table[s * table_stride +
+ * p / page_tokens]. start, cached and table are device arrays, so a recorded
+ * pass reads their values of each replay; max_tokens is the most tokens of the
+ * call that any sequence has (or a bound of it). Nothing is accessed outside
+ * the cache whatever the arrays hold: a page number past the cache is never
+ * written (reading, it stands for the last page), positions past the table are
+ * left out, and so are a sequence's tokens past max_tokens (their outputs are
+ * not written). */
+typedef struct mx4_batch {
+    uint32_t seqs, tokens, max_tokens, table_stride;
+    const uint32_t *start;
+    const uint32_t *cached;
+    const uint32_t *table;
+} mx4_batch;
+
+/* out_dev [positions][head_dim] f32: cos(p t_i), then sin(p t_i), for i <
+ * head_dim / 2, t_i = theta^(-2 i / head_dim) (the angles of
+ * engine/src/gpu.metal:82-97), computed in 64 bits. head_dim even. */
+mx4_status mx4_rope_table(mx4_context *ctx, uint32_t positions, uint32_t head_dim, double theta, float *out_dev);
+
+/* The rows that mx4_qk_norm_rope reads: token t's q heads are q[t * q_stride ..
+ * + q_heads * head_dim), its k and v heads likewise (strides in elements, 0:
+ * packed; a fused product's rows are three pointers and one stride). f32 or bf16
+ * (an mx4_dtype), every row 16-byte aligned. q_norm, k_norm: bf16 [head_dim]
+ * norm weights (NULL: no norm). rope: mx4_rope_table's rows (NULL: no rotation;
+ * a position past the table takes its last row). positions [tokens]: each
+ * token's position (NULL: its place in the sequence; in a drafted tree, its
+ * depth behind the cached tokens). */
+typedef struct mx4_qkv {
+    const void *q, *k, *v;
+    uint64_t q_stride, k_stride, v_stride;
+    const uint16_t *q_norm, *k_norm;
+    const float *rope;
+    const uint32_t *positions;
+    uint32_t rope_positions, q_heads;
+    int32_t type;
+    float eps;
+} mx4_qkv;
+
+/* Norm of every q and k head (engine/src/gpu.metal:57-78: x w / sqrt(mean(x^2)
+ * + eps)), the rotation of the pairs (i, i + head_dim / 2) by position
+ * (engine/src/gpu.metal:82-97), and the new keys and values written to layer
+ * `layer` of the cache at the tokens' places, in one launch. q_out_dev: bf16
+ * rows of q_heads * head_dim, q_out_stride elements apart (0: packed).
+ * Arithmetic in f32, one rounding to bf16. */
+mx4_status mx4_qk_norm_rope(mx4_context *ctx, const mx4_qkv *in, const mx4_batch *batch, const mx4_kv_cache *cache,
+                            uint32_t layer, uint16_t *q_out_dev, uint64_t q_out_stride);
+
+/* Attention of the call's queries over their sequences' cached and new keys
+ * (engine/src/gpu.metal:101-151; mx4_qk_norm_rope has put the new ones into the
+ * cache): q_dev and out_dev bf16 rows of q_heads * head_dim (strides in
+ * elements, 0: packed; rows 16-byte aligned), q_heads a multiple of the cache's
+ * kv_heads. tree_dev NULL: new token i of a sequence sees the cached tokens and
+ * the new ones 0 .. i. Otherwise tree_dev [tokens][tree_words] are masks: token
+ * t sees the cached tokens and the new token j of its sequence if bit j % 64 of
+ * tree_dev[t * tree_words + j / 64] is set (its own bit included). A token that
+ * sees no key gets zeros; keys it does not see have no part in it, whatever
+ * they hold. scale multiplies q . k (0: 1 / sqrt(head_dim)). Scores, the running
+ * maximum and sum and the output are f32; the weights meet v rounded to bf16.
+ * Uses the context's split scratch, allocates nothing. */
+mx4_status mx4_attention(mx4_context *ctx, const uint16_t *q_dev, uint64_t q_stride, uint32_t q_heads,
+                         const mx4_batch *batch, const mx4_kv_cache *cache, uint32_t layer, const uint64_t *tree_dev,
+                         uint32_t tree_words, float scale, uint16_t *out_dev, uint64_t out_stride);
+
+/* Copies pages in every layer, keys and values: pairs_dev [count][2] of
+ * (source, destination). No destination is also a source or named twice (a
+ * pair naming a page past the cache is left out). */
+mx4_status mx4_cache_copy_pages(mx4_context *ctx, const mx4_kv_cache *cache, const uint32_t *pairs_dev, uint32_t count);
+
+/* After a verify step: in every layer, the new token kept_dev[s * max_kept + j]
+ * of sequence s becomes its new token j, for j < kept_count_dev[s] -- the
+ * accepted path of a tree moves to the front, behind the cached tokens. A list
+ * ascends strictly (a path does, where parents come before children); entries
+ * that are no new token of the sequence are left out. */
+mx4_status mx4_cache_keep(mx4_context *ctx, const mx4_kv_cache *cache, const mx4_batch *batch,
+                          const uint32_t *kept_dev, const uint32_t *kept_count_dev, uint32_t max_kept);
+
+/* Which pages belong to which sequence: host bookkeeping, needs no GPU. Pages
+ * are counted, so forked sequences share what neither has written since. Every
+ * call either does all it says or changes nothing. Not thread-safe. */
+typedef struct mx4_pages mx4_pages;
+mx4_status mx4_pages_create(uint32_t pages, uint32_t page_tokens, mx4_pages **out);
+void mx4_pages_destroy(mx4_pages *pages);
+mx4_status mx4_pages_free_count(const mx4_pages *pages, uint32_t *out);
+/* A new, empty sequence. */
+mx4_status mx4_pages_open(mx4_pages *pages, uint32_t *seq);
+/* A sequence with the same tokens on the same pages. */
+mx4_status mx4_pages_fork(mx4_pages *pages, uint32_t seq, uint32_t *child);
+/* Makes the positions from .. to - 1 of a sequence writable (from at most its
+ * length), which then has `to` tokens: what it had from `from` on is given up,
+ * pages it lacks are added, shared ones it is about to write are replaced. If
+ * the first of these holds earlier tokens too, they have to be copied first:
+ * then *copies is 1 and pair its (source, destination) for mx4_cache_copy_pages,
+ * else 0. MX4_ERR_NO_MEMORY when too few pages are free. */
+mx4_status mx4_pages_write(mx4_pages *pages, uint32_t seq, uint32_t from, uint32_t to, uint32_t pair[2],
+                           uint32_t *copies);
+/* Cuts a sequence to `tokens` tokens (no more than it has) and frees the pages
+ * behind them that no other sequence holds. */
+mx4_status mx4_pages_trim(mx4_pages *pages, uint32_t seq, uint32_t tokens);
+mx4_status mx4_pages_close(mx4_pages *pages, uint32_t seq);
+/* The sequence's length and page numbers (table NULL: the numbers are only
+ * counted); MX4_ERR_LENGTH if there are more than `capacity`. */
+mx4_status mx4_pages_table(const mx4_pages *pages, uint32_t seq, uint32_t *tokens, uint32_t *table, uint32_t capacity,
+                           uint32_t *count);
+/* Renumbers the pages in use to 0 .. n - 1: pairs [*count][2] are the copies
+ * that mx4_cache_copy_pages then has to make (no destination is a source).
+ * MX4_ERR_LENGTH, with *count set, if there are more than `capacity`. */
+mx4_status mx4_pages_compact(mx4_pages *pages, uint32_t *pairs, uint32_t capacity, uint32_t *count);
+
 /* Synthetic inputs (the reference defines none): element i of stream `seed`
  * is bf16(RNE(f32(RNE(sigma * z_i)))) with z_i a Box-Muller normal from
  * SplitMix64 outputs 2i and 2i+1. */

@@ -1,0 +1,226 @@
+// cache.hip -- what stands between the q|k|v projections and the attention of a
+// step, and what moves a cache's pages: per-head norms with the rotation and
+// the cache write in one pass, page copies, and the accepted tokens of a tree.
+#include <hip/hip_runtime.h>
+
+#include "cache_device.h"
+
+namespace mx4 {
+
+// ------------------------------------------------------------- rope table
+
+// In 64 bits: position 40000 times an angle of 1 has to keep its fraction.
+__global__ void rope_table_kernel(uint32_t positions, uint32_t half, double log_theta, float* out) {
+    const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= (uint64_t)positions * half) return;
+    const uint32_t p = (uint32_t)(i / half), j = (uint32_t)(i % half);
+    double s, c;
+    sincos(p * exp(-log_theta * j / half), &s, &c);
+    out[(uint64_t)p * 2 * half + j] = (float)c;
+    out[(uint64_t)p * 2 * half + half + j] = (float)s;
+}
+
+hipError_t launch_rope_table(uint32_t positions, uint32_t head_dim, double theta, float* out, hipStream_t s) {
+    const uint64_t n = (uint64_t)positions * (head_dim / 2);
+    rope_table_kernel<<<dim3((uint32_t)((n + 255) / 256)), dim3(256), 0, s>>>(positions, head_dim / 2, log(theta), out);
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------------- norm + rotation + cache write
+
+// A head of D values is D / 8 lanes of 8. For q and k, with u = x w / sqrt(mean(x^2) + eps)
+// and lane c's partner D / 16 lanes away holding the other half's values:
+//   y[i] = u[i] cos - u[i + D/2] sin,  y[i + D/2] = u[i + D/2] cos + u[i] sin.
+// k goes to its place in the cache, v too (unchanged but for the type), q to q_out.
+template <int D, bool XBF16>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
+    constexpr int LANES = D / 8, PER_WAVE = 64 / LANES, PER_BLOCK = 4 * PER_WAVE;
+    const uint32_t t = blockIdx.x;
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t c = lane % LANES;
+    const uint32_t heads = a.q_heads + 2 * a.cache.kv_heads;
+
+    const uint32_t s = sequence_of(a.step.start, a.step.seqs, t);
+    uint32_t slot = 0xffffffffu, position = 0;
+    uint64_t row = 0;
+    if (s < a.step.seqs) {
+        slot = a.step.cached[s] + (t - a.step.start[s]);
+        position = slot;
+        const uint32_t entry = slot >> a.cache.page_shift;
+        uint32_t page = a.cache.pages;
+        if (entry < a.step.table_stride) page = a.step.table[(uint64_t)s * a.step.table_stride + entry];
+        if (page < a.cache.pages)
+            row = (((uint64_t)page * a.cache.kv_heads) << a.cache.page_shift) + (slot & ((1u << a.cache.page_shift) - 1));
+        else
+            slot = 0xffffffffu;
+    }
+    if (a.positions) position = a.positions[t];
+
+    f32x4 cs[2] = {}, sn[2] = {};
+    if (a.table) {
+        const float* at = a.table + (uint64_t)min(position, a.table_positions - 1) * D + (c * 8) % (D / 2);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            cs[i] = reinterpret_cast<const f32x4*>(at)[i];
+            sn[i] = reinterpret_cast<const f32x4*>(at + D / 2)[i];
+        }
+    }
+    for (uint32_t h = blockIdx.y * PER_BLOCK + wave * PER_WAVE + lane / LANES; h < heads; h += gridDim.y * PER_BLOCK) {
+        const bool is_q = h < a.q_heads, is_k = !is_q && h < a.q_heads + a.cache.kv_heads;
+        const uint32_t kv = is_q ? 0 : is_k ? h - a.q_heads : h - a.q_heads - a.cache.kv_heads;
+        const void* from = is_q ? a.q : is_k ? a.k : a.v;
+        const uint64_t at = t * (is_q ? a.q_stride : is_k ? a.k_stride : a.v_stride) + (is_q ? h : kv) * D + c * 8;
+        float x[8];
+        if (XBF16) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(from) + at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[2 * i] = __uint_as_float(w[i] << 16);
+                x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        } else {
+            const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(from) + at);
+            const f32x4 lo = p[0], hi = p[1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = lo[i];
+                x[4 + i] = hi[i];
+            }
+        }
+        const uint16_t* norm = is_q ? a.q_norm : is_k ? a.k_norm : nullptr;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(x[i], x[i], sum);
+#pragma unroll
+        for (int off = 1; off < LANES; off *= 2) sum += __shfl_xor(sum, off);
+        if (norm) {
+            const float r = 1.0f / sqrtf(sum / D + a.eps);
+            const u32x4 w = *reinterpret_cast<const u32x4*>(norm + c * 8);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[2 * i] *= r * __uint_as_float(w[i] << 16);
+                x[2 * i + 1] *= r * __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __shfl_xor(x[i], LANES / 2);
+        const bool turn = a.table && (is_q || is_k);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float other = c < LANES / 2 ? -y[i] : y[i];
+            y[i] = turn ? x[i] * cs[i / 4][i % 4] + other * sn[i / 4][i % 4] : x[i];
+        }
+        bf16x8 o;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = (__bf16)y[i];  // the one rounding
+        if (is_q) {
+            *reinterpret_cast<bf16x8*>(a.q_out + t * a.out_stride + h * D + c * 8) = o;
+        } else if (slot != 0xffffffffu) {
+            uint16_t* to = (is_k ? a.cache.k : a.cache.v) + (row + ((uint64_t)kv << a.cache.page_shift)) * D + c * 8;
+            *reinterpret_cast<bf16x8*>(to) = o;
+        }
+    }
+}
+
+hipError_t launch_qk_norm_rope(const RopeArgs& a, int cus) {
+    const uint32_t heads = a.q_heads + 2 * a.cache.kv_heads, per_block = 4 * 64 / (a.cache.head_dim / 8);
+    uint32_t y = (heads + per_block - 1) / per_block;
+    if (a.step.tokens >= 4u * cus) y = 1;
+    const dim3 grid(a.step.tokens, y);
+#define MX4_ROPE(D)                                                                               \
+    if (a.cache.head_dim == D) {                                                                  \
+        if (a.x_bf16) qk_norm_rope_kernel<D, true><<<grid, dim3(256), 0, a.stream>>>(a);          \
+        else qk_norm_rope_kernel<D, false><<<grid, dim3(256), 0, a.stream>>>(a);                  \
+    }
+    MX4_ROPE(64)
+    MX4_ROPE(128)
+    MX4_ROPE(256)
+#undef MX4_ROPE
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------------- page copies
+
+// Block (chunk, pair, layer and side): 16-byte pieces, four in flight a thread.
+__global__ __launch_bounds__(256) void copy_pages_kernel(CacheView c, const uint32_t* pairs, uint32_t pieces) {
+    const uint32_t src = pairs[2 * blockIdx.y], dst = pairs[2 * blockIdx.y + 1];
+    if (src >= c.pages || dst >= c.pages || src == dst) return;
+    uint16_t* base = (blockIdx.z & 1 ? c.v : c.k) + (blockIdx.z >> 1) * c.layer_stride;
+    const u32x4* from = reinterpret_cast<const u32x4*>(base) + (uint64_t)src * pieces;
+    u32x4* to = reinterpret_cast<u32x4*>(base) + (uint64_t)dst * pieces;
+    const uint32_t at = blockIdx.x * 1024 + threadIdx.x;
+    u32x4 w[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+        if (at + i * 256 < pieces) w[i] = from[at + i * 256];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+        if (at + i * 256 < pieces) to[at + i * 256] = w[i];
+}
+
+hipError_t launch_copy_pages(const CacheView& c, const uint32_t* pairs, uint32_t count, int cus, hipStream_t s) {
+    const uint32_t pieces = (uint32_t)(((uint64_t)c.kv_heads << c.page_shift) * c.head_dim / 8);
+    for (uint32_t at = 0; at < count; at += 65535) {
+        const uint32_t n = count - at < 65535 ? count - at : 65535;
+        copy_pages_kernel<<<dim3((pieces + 1023) / 1024, n, 2 * c.layers), dim3(256), 0, s>>>(c, pairs + 2 * (uint64_t)at, pieces);
+    }
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------------- kept tokens
+
+// A wave moves one head's rows of one sequence, layer and side, in place. The
+// list ascends, so kept[j] >= j: a row written by a pass is never read by a
+// later one, and within a pass every read ends before the first write.
+template <int D>
+__global__ __launch_bounds__(256) void keep_kernel(CacheView c, StepView st, const uint32_t* kept,
+                                                   const uint32_t* kept_count, uint32_t max_kept) {
+    constexpr int LANES = D / 8, ROWS = 64 / LANES, DEEP = 4;
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t head = blockIdx.x * 4 + (threadIdx.x >> 6), s = blockIdx.y;
+    if (head >= c.kv_heads) return;
+    uint32_t first, fresh;
+    tokens_of(st, s, first, fresh);
+    const uint32_t count = min(min(kept_count[s], max_kept), fresh), before = st.cached[s];
+    uint16_t* base = (blockIdx.z & 1 ? c.v : c.k) + (blockIdx.z >> 1) * c.layer_stride;
+    const uint32_t* table = st.table + (uint64_t)s * st.table_stride;
+    const uint32_t mask = (1u << c.page_shift) - 1;
+    auto place = [&](uint32_t position, uint64_t& at) {
+        const uint32_t entry = position >> c.page_shift;
+        const uint32_t page = entry < st.table_stride ? table[entry] : c.pages;
+        at = ((((uint64_t)page * c.kv_heads + head) << c.page_shift) + (position & mask)) * D + (lane % LANES) * 8;
+        return page < c.pages;
+    };
+    for (uint32_t j0 = 0; j0 < count; j0 += ROWS * DEEP) {
+        u32x4 w[DEEP];
+        bool move[DEEP];
+#pragma unroll
+        for (int i = 0; i < DEEP; ++i) {
+            const uint32_t j = j0 + i * ROWS + lane / LANES;
+            const uint32_t from = j < count ? kept[(uint64_t)s * max_kept + j] : j;
+            uint64_t at = 0;
+            move[i] = j < count && from != j && from < fresh && place(before + from, at);
+            if (move[i]) w[i] = *reinterpret_cast<const u32x4*>(base + at);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < DEEP; ++i) {
+            const uint32_t j = j0 + i * ROWS + lane / LANES;
+            uint64_t at = 0;
+            if (move[i] && place(before + j, at)) *reinterpret_cast<u32x4*>(base + at) = w[i];
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+}
+
+hipError_t launch_keep(const CacheView& c, const StepView& st, const uint32_t* kept, const uint32_t* kept_count,
+                       uint32_t max_kept, hipStream_t s) {
+    const dim3 grid((c.kv_heads + 3) / 4, st.seqs, 2 * c.layers);
+    if (c.head_dim == 64) keep_kernel<64><<<grid, dim3(256), 0, s>>>(c, st, kept, kept_count, max_kept);
+    if (c.head_dim == 128) keep_kernel<128><<<grid, dim3(256), 0, s>>>(c, st, kept, kept_count, max_kept);
+    if (c.head_dim == 256) keep_kernel<256><<<grid, dim3(256), 0, s>>>(c, st, kept, kept_count, max_kept);
+    return hipGetLastError();
+}
+
+}  // namespace mx4

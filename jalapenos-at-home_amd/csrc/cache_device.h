@@ -1,0 +1,40 @@
+// cache_device.h -- what the kernels over a paged key/value cache share: where
+// a step's token and a sequence's position live. Everything read from device
+// memory (starts, lengths, page numbers) is bounded before it becomes an
+// address, so a wrong number gives wrong values and no access out of range.
+#pragma once
+
+#include "mx4_device.h"
+#include "mx4_kernels.h"
+
+namespace mx4 {
+
+// Sequence of token t: how many sequences end at or before it (seqs: none owns
+// it). Called by a whole wave, 64 ends a probe.
+__device__ __forceinline__ uint32_t sequence_of(const uint32_t* start, uint32_t seqs, uint32_t t) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t lo = 0, n = seqs;
+    while (n > 64) {
+        const uint32_t step = (n + 63) / 64, at = (lane + 1) * step;
+        const uint32_t whole = __popcll(__ballot(at <= n && start[lo + (at <= n ? at : n)] <= t));
+        lo += whole * step;
+        n -= whole * step;
+        if (n > step) n = step;
+    }
+    return lo + __popcll(__ballot(lane < n && start[lo + (lane < n ? lane + 1 : n)] <= t));
+}
+
+// First token and number of tokens of a sequence in this call.
+__device__ __forceinline__ void tokens_of(const StepView& st, uint32_t s, uint32_t& first, uint32_t& count) {
+    const uint32_t a = min(st.start[s], st.tokens), b = min(st.start[s + 1], st.tokens);
+    first = a;
+    count = b > a ? min(b - a, st.max_tokens) : 0;
+}
+
+// Positions that a sequence's row of the page table can hold, at most 2^31.
+__device__ __forceinline__ uint32_t table_room(const StepView& st, uint32_t page_shift) {
+    const uint64_t room = (uint64_t)st.table_stride << page_shift;
+    return room < 0x80000000ull ? (uint32_t)room : 0x80000000u;
+}
+
+}  // namespace mx4

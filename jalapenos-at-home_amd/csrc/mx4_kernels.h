@@ -219,4 +219,66 @@ double mfma_ceiling_flops(int shape, uint32_t iters, uint32_t grid);
 hipError_t launch_mfma_ceiling(int shape, uint32_t iters, bool random, uint32_t grid, uint64_t* clocks, float* sink,
                                hipStream_t s);
 
+// ---- a paged key/value cache and the step over it (include/mx4.h) ----
+// One layer's pages [pages][kv_heads][page][head_dim] (several layers' for the
+// copies: layer_stride elements apart).
+struct CacheView {
+    uint16_t* k;
+    uint16_t* v;
+    uint64_t layer_stride;
+    uint32_t layers, pages, kv_heads, page_shift, head_dim;
+};
+// The step's tokens: sequence s has tokens start[s] .. start[s + 1] - 1 of the
+// call, which come after the cached[s] it has; its position p lives in page
+// table[s * table_stride + p / page].
+struct StepView {
+    const uint32_t* start;
+    const uint32_t* cached;
+    const uint32_t* table;
+    uint32_t table_stride, seqs, tokens, max_tokens;
+};
+
+// cos | sin of position * theta^(-2 i / head_dim), rows of head_dim floats
+hipError_t launch_rope_table(uint32_t positions, uint32_t head_dim, double theta, float* out, hipStream_t s);
+struct RopeArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    uint64_t q_stride, k_stride, v_stride;  // elements
+    const uint16_t* q_norm;
+    const uint16_t* k_norm;
+    float eps;
+    const float* table;
+    uint32_t table_positions;
+    const uint32_t* positions;
+    uint16_t* q_out;
+    uint64_t out_stride;
+    uint32_t q_heads;
+    bool x_bf16;
+    CacheView cache;  // k, v at the layer
+    StepView step;
+    hipStream_t stream;
+};
+hipError_t launch_qk_norm_rope(const RopeArgs& a, int cus);
+// pairs [count][2]: page pairs[2 i] of every layer to page pairs[2 i + 1]
+hipError_t launch_copy_pages(const CacheView& c, const uint32_t* pairs, uint32_t count, int cus, hipStream_t s);
+// kept [seqs][max_kept], ascending: new token kept[s][j] of sequence s becomes its new token j
+hipError_t launch_keep(const CacheView& c, const StepView& st, const uint32_t* kept, const uint32_t* kept_count,
+                       uint32_t max_kept, hipStream_t s);
+struct AttentionArgs {
+    const uint16_t* q;
+    uint16_t* out;
+    uint64_t q_stride, out_stride;  // elements
+    uint32_t q_heads;
+    const uint64_t* tree;  // [tokens][tree_words], or null: chains
+    uint32_t tree_words;
+    float scale;
+    CacheView cache;  // k, v at the layer
+    StepView step;
+    float* part;  // scratch of the joined splits
+    uint64_t part_bytes;
+    hipStream_t stream;
+};
+hipError_t launch_attention(const AttentionArgs& a, int cus);
+
 }  // namespace mx4

@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -161,6 +162,7 @@ constexpr uint32_t kSplitPartTiles = 4096;
 constexpr uint32_t kSplitCounts = 4096;
 
 namespace mx4 {
+mx4_status report(mx4_status st, const char* message) { return fail(st, "%s", message); }
 hipError_t launch_fill_u32(uint32_t* p, uint32_t count, uint32_t value, hipStream_t s);
 }
 
@@ -1429,6 +1431,176 @@ mx4_status mx4_argmax_rows(mx4_context* ctx, const float* x, uint32_t rows, uint
     hipError_t e = mx4::launch_argmax_rows(x, rows, width, out, ctx->am_partial, kArgmaxPartials, ctx->cus,
                                            ctx->stream);
     if (e != hipSuccess) return fail(MX4_ERR_DEVICE, "argmax launch failed: %s", hipGetErrorString(e));
+    return MX4_OK;
+}
+
+namespace {
+
+bool aligned(const void* p, uintptr_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+
+// The cache as the kernels see it, k and v at `layer` (layer 0 and all layers
+// for the copies).
+mx4_status check_cache(const mx4_kv_cache* c, uint32_t layer, mx4::CacheView* out) {
+    if (!c || !c->k || !c->v) return fail(MX4_ERR_ARGUMENT, "null cache");
+    if (!aligned(c->k, 16) || !aligned(c->v, 16)) return fail(MX4_ERR_ARGUMENT, "the cache must be 16-byte aligned");
+    if (c->layers == 0 || c->pages == 0 || c->kv_heads == 0)
+        return fail(MX4_ERR_SHAPE, "a cache has at least one layer, page and head");
+    if (c->layers > 32767 || c->kv_heads > 65535) return fail(MX4_ERR_TOO_LARGE, "at most 32767 layers and 65535 heads");
+    if (c->page_tokens < 16 || c->page_tokens > 4096 || (c->page_tokens & (c->page_tokens - 1)) != 0)
+        return fail(MX4_ERR_SHAPE, "page_tokens must be a power of two from 16 to 4096, got %u", c->page_tokens);
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+        return fail(MX4_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256, got %u", c->head_dim);
+    if (layer >= c->layers) return fail(MX4_ERR_ARGUMENT, "layer %u of a cache of %u", layer, c->layers);
+    const unsigned __int128 packed = (unsigned __int128)c->pages * c->kv_heads * c->page_tokens * c->head_dim;
+    if (packed * c->layers >> 62) return fail(MX4_ERR_TOO_LARGE, "cache too large");
+    if (c->layer_stride != 0 && (c->layer_stride < packed || c->layer_stride % 8 != 0 || c->layer_stride >> 47))
+        return fail(MX4_ERR_SHAPE, "layer_stride must be a multiple of 8 that holds a layer");
+    uint32_t shift = 0;
+    while ((1u << shift) < c->page_tokens) ++shift;
+    const uint64_t stride = c->layer_stride ? c->layer_stride : (uint64_t)packed;
+    *out = {c->k + layer * stride, c->v + layer * stride, stride, c->layers, c->pages, c->kv_heads, shift, c->head_dim};
+    return MX4_OK;
+}
+
+mx4_status check_batch(const mx4_batch* b, mx4::StepView* out) {
+    if (!b || !b->start || !b->cached || !b->table) return fail(MX4_ERR_ARGUMENT, "null batch");
+    if (!aligned(b->start, 4) || !aligned(b->cached, 4) || !aligned(b->table, 4))
+        return fail(MX4_ERR_ARGUMENT, "the batch's arrays must be 4-byte aligned");
+    if (b->seqs == 0 || b->table_stride == 0) return fail(MX4_ERR_SHAPE, "a batch has at least one sequence and one page a row");
+    if (b->seqs > 65535) return fail(MX4_ERR_TOO_LARGE, "at most 65535 sequences");
+    if (b->tokens > (1u << 30)) return fail(MX4_ERR_TOO_LARGE, "at most 2^30 tokens");
+    if (b->tokens != 0 && (b->max_tokens == 0 || b->max_tokens > b->tokens))
+        return fail(MX4_ERR_ARGUMENT, "max_tokens must be 1 .. tokens");
+    *out = {b->start, b->cached, b->table, b->table_stride, b->seqs, b->tokens, b->max_tokens};
+    return MX4_OK;
+}
+
+// A row stride in elements of `size` bytes: 0 is packed; rows stay 16-byte aligned.
+bool row_stride(uint64_t given, uint64_t width, uint32_t size, uint64_t* out) {
+    *out = given ? given : width;
+    return *out >= width && *out >> 32 == 0 && *out * size % 16 == 0;
+}
+
+}  // namespace
+
+mx4_status mx4_rope_table(mx4_context* ctx, uint32_t positions, uint32_t head_dim, double theta, float* out) {
+    if (!ctx || !out) return fail(MX4_ERR_ARGUMENT, "null argument");
+    if (positions == 0 || head_dim == 0 || head_dim % 2 != 0)
+        return fail(MX4_ERR_SHAPE, "a rotation table needs positions and an even head_dim");
+    if ((uint64_t)positions * head_dim >> 36) return fail(MX4_ERR_TOO_LARGE, "rotation table too large");
+    if (!(theta > 0.0) || theta > 1e300) return fail(MX4_ERR_ARGUMENT, "theta must be positive and finite");
+    if (!aligned(out, 16)) return fail(MX4_ERR_ARGUMENT, "the table must be 16-byte aligned");
+    DeviceGuard g(ctx->device);
+    const hipError_t e = mx4::launch_rope_table(positions, head_dim, theta, out, ctx->stream);
+    if (e != hipSuccess) return fail(MX4_ERR_DEVICE, "rotation table launch failed: %s", hipGetErrorString(e));
+    return MX4_OK;
+}
+
+mx4_status mx4_qk_norm_rope(mx4_context* ctx, const mx4_qkv* in, const mx4_batch* batch, const mx4_kv_cache* cache,
+                            uint32_t layer, uint16_t* q_out, uint64_t q_out_stride) {
+    if (!ctx || !in || !in->q || !in->k || !in->v || !q_out) return fail(MX4_ERR_ARGUMENT, "null argument");
+    if (in->type != MX4_F32 && in->type != MX4_BF16) return fail(MX4_ERR_ARGUMENT, "bad activation dtype %d", (int)in->type);
+    mx4::RopeArgs a{};
+    mx4_status st = check_cache(cache, layer, &a.cache);
+    if (st != MX4_OK) return st;
+    st = check_batch(batch, &a.step);
+    if (st != MX4_OK) return st;
+    if (in->q_heads == 0 || in->q_heads > 65535) return fail(MX4_ERR_SHAPE, "q_heads must be 1 .. 65535");
+    if (!(in->eps >= 0.0f) || in->eps > 1e30f) return fail(MX4_ERR_ARGUMENT, "eps must be finite and not negative");
+    if (in->rope && in->rope_positions == 0) return fail(MX4_ERR_SHAPE, "empty rotation table");
+    const uint32_t size = in->type == MX4_BF16 ? 2 : 4, d = cache->head_dim;
+    if (!row_stride(in->q_stride, (uint64_t)in->q_heads * d, size, &a.q_stride) ||
+        !row_stride(in->k_stride, (uint64_t)cache->kv_heads * d, size, &a.k_stride) ||
+        !row_stride(in->v_stride, (uint64_t)cache->kv_heads * d, size, &a.v_stride) ||
+        !row_stride(q_out_stride, (uint64_t)in->q_heads * d, 2, &a.out_stride))
+        return fail(MX4_ERR_SHAPE, "a stride is shorter than its row, breaks its alignment or is past 2^32 elements");
+    if (!aligned(in->q, 16) || !aligned(in->k, 16) || !aligned(in->v, 16) || !aligned(q_out, 16) ||
+        !aligned(in->q_norm, 16) || !aligned(in->k_norm, 16) || !aligned(in->rope, 16))
+        return fail(MX4_ERR_ARGUMENT, "q, k, v, the norm weights, the table and the output must be 16-byte aligned");
+    if (!aligned(in->positions, 4)) return fail(MX4_ERR_ARGUMENT, "positions must be 4-byte aligned");
+    if (a.step.tokens == 0) return MX4_OK;
+    a.q = in->q;
+    a.k = in->k;
+    a.v = in->v;
+    a.q_norm = in->q_norm;
+    a.k_norm = in->k_norm;
+    a.eps = in->eps;
+    a.table = in->rope;
+    a.table_positions = in->rope_positions;
+    a.positions = in->positions;
+    a.q_out = q_out;
+    a.q_heads = in->q_heads;
+    a.x_bf16 = in->type == MX4_BF16;
+    a.stream = ctx->stream;
+    DeviceGuard g(ctx->device);
+    const hipError_t e = mx4::launch_qk_norm_rope(a, ctx->cus);
+    if (e != hipSuccess) return fail(MX4_ERR_DEVICE, "norm and rotation launch failed: %s", hipGetErrorString(e));
+    return MX4_OK;
+}
+
+mx4_status mx4_attention(mx4_context* ctx, const uint16_t* q, uint64_t q_stride, uint32_t q_heads,
+                         const mx4_batch* batch, const mx4_kv_cache* cache, uint32_t layer, const uint64_t* tree,
+                         uint32_t tree_words, float scale, uint16_t* out, uint64_t out_stride) {
+    if (!ctx || !q || !out) return fail(MX4_ERR_ARGUMENT, "null argument");
+    mx4::AttentionArgs a{};
+    mx4_status st = check_cache(cache, layer, &a.cache);
+    if (st != MX4_OK) return st;
+    st = check_batch(batch, &a.step);
+    if (st != MX4_OK) return st;
+    if (q_heads == 0 || q_heads > 65535 || q_heads % cache->kv_heads != 0)
+        return fail(MX4_ERR_SHAPE, "q_heads must be a multiple of the cache's %u heads, at most 65535", cache->kv_heads);
+    if (!row_stride(q_stride, (uint64_t)q_heads * cache->head_dim, 2, &a.q_stride) ||
+        !row_stride(out_stride, (uint64_t)q_heads * cache->head_dim, 2, &a.out_stride))
+        return fail(MX4_ERR_SHAPE, "a stride is shorter than its row, breaks its alignment or is past 2^32 elements");
+    if (!aligned(q, 16) || !aligned(out, 16)) return fail(MX4_ERR_ARGUMENT, "q and out must be 16-byte aligned");
+    if (tree && !aligned(tree, 8)) return fail(MX4_ERR_ARGUMENT, "the tree masks must be 8-byte aligned");
+    if (tree && (uint64_t)tree_words * 64 < a.step.max_tokens)
+        return fail(MX4_ERR_SHAPE, "%u mask words hold no tree of %u tokens", tree_words, a.step.max_tokens);
+    if (!(scale >= 0.0f) || scale > 1e30f) return fail(MX4_ERR_ARGUMENT, "scale must be positive and finite (0: default)");
+    if (a.step.tokens == 0) return MX4_OK;
+    a.q = q;
+    a.out = out;
+    a.q_heads = q_heads;
+    a.tree = tree;
+    a.tree_words = tree_words;
+    a.scale = scale > 0.0f ? scale : 1.0f / std::sqrt((float)cache->head_dim);
+    a.part = ctx->split_part;
+    a.part_bytes = kSplitPartBytes;
+    a.stream = ctx->stream;
+    DeviceGuard g(ctx->device);
+    const hipError_t e = mx4::launch_attention(a, ctx->cus);
+    if (e != hipSuccess) return fail(MX4_ERR_DEVICE, "attention launch failed: %s", hipGetErrorString(e));
+    return MX4_OK;
+}
+
+mx4_status mx4_cache_copy_pages(mx4_context* ctx, const mx4_kv_cache* cache, const uint32_t* pairs, uint32_t count) {
+    if (!ctx || (!pairs && count)) return fail(MX4_ERR_ARGUMENT, "null argument");
+    mx4::CacheView c;
+    mx4_status st = check_cache(cache, 0, &c);
+    if (st != MX4_OK) return st;
+    if (!aligned(pairs, 4)) return fail(MX4_ERR_ARGUMENT, "pairs must be 4-byte aligned");
+    if (count == 0) return MX4_OK;
+    DeviceGuard g(ctx->device);
+    const hipError_t e = mx4::launch_copy_pages(c, pairs, count, ctx->cus, ctx->stream);
+    if (e != hipSuccess) return fail(MX4_ERR_DEVICE, "page copy launch failed: %s", hipGetErrorString(e));
+    return MX4_OK;
+}
+
+mx4_status mx4_cache_keep(mx4_context* ctx, const mx4_kv_cache* cache, const mx4_batch* batch, const uint32_t* kept,
+                          const uint32_t* kept_count, uint32_t max_kept) {
+    if (!ctx || !kept || !kept_count) return fail(MX4_ERR_ARGUMENT, "null argument");
+    mx4::CacheView c;
+    mx4_status st = check_cache(cache, 0, &c);
+    if (st != MX4_OK) return st;
+    mx4::StepView step;
+    st = check_batch(batch, &step);
+    if (st != MX4_OK) return st;
+    if (!aligned(kept, 4) || !aligned(kept_count, 4)) return fail(MX4_ERR_ARGUMENT, "the lists must be 4-byte aligned");
+    if (max_kept > (1u << 30)) return fail(MX4_ERR_TOO_LARGE, "at most 2^30 kept tokens");
+    if (max_kept == 0 || step.tokens == 0) return MX4_OK;
+    DeviceGuard g(ctx->device);
+    const hipError_t e = mx4::launch_keep(c, step, kept, kept_count, max_kept, ctx->stream);
+    if (e != hipSuccess) return fail(MX4_ERR_DEVICE, "kept tokens' launch failed: %s", hipGetErrorString(e));
     return MX4_OK;
 }
 

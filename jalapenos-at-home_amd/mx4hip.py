@@ -28,6 +28,7 @@ ERR_UNSUPPORTED = 9
 F32, BF16 = 0, 1
 PATH_AUTO, PATH_GEMV, PATH_SKINNY, PATH_GENERIC, PATH_PREFILL, PATH_GEMM = 0, 1, 2, 3, 4, 5
 ACT_MXFP4, ACT_MXFP8 = 1, 2
+STREAM_LEGACY = 1  # hipStreamLegacy: the device's default stream, for Context.set_stream
 
 _vp = ctypes.c_void_p
 _u8p = ctypes.POINTER(ctypes.c_uint8)
@@ -36,6 +37,7 @@ _u16p = ctypes.POINTER(ctypes.c_uint16)
 _u32 = ctypes.c_uint32
 _u64 = ctypes.c_uint64
 _int = ctypes.c_int
+_u32p = ctypes.POINTER(_u32)
 
 SIGNATURES = {
     "qwen_hip_create": (_vp, []),
@@ -100,6 +102,21 @@ SIGNATURES = {
     "mx4_timer_begin": (_int, [_vp]),
     "mx4_timer_end": (_int, [_vp, ctypes.POINTER(ctypes.c_double)]),
     "mx4_decode_table": (_int, [_vp, _int, _vp]),
+    "mx4_rope_table": (_int, [_vp, _u32, _u32, ctypes.c_double, _vp]),
+    "mx4_qk_norm_rope": (_int, [_vp, _vp, _vp, _vp, _u32, _vp, _u64]),
+    "mx4_attention": (_int, [_vp, _vp, _u64, _u32, _vp, _vp, _u32, _vp, _u32, ctypes.c_float, _vp, _u64]),
+    "mx4_cache_copy_pages": (_int, [_vp, _vp, _vp, _u32]),
+    "mx4_cache_keep": (_int, [_vp, _vp, _vp, _vp, _vp, _u32]),
+    "mx4_pages_create": (_int, [_u32, _u32, ctypes.POINTER(_vp)]),
+    "mx4_pages_destroy": (None, [_vp]),
+    "mx4_pages_free_count": (_int, [_vp, _u32p]),
+    "mx4_pages_open": (_int, [_vp, _u32p]),
+    "mx4_pages_fork": (_int, [_vp, _u32, _u32p]),
+    "mx4_pages_write": (_int, [_vp, _u32, _u32, _u32, _u32p, _u32p]),
+    "mx4_pages_trim": (_int, [_vp, _u32, _u32]),
+    "mx4_pages_close": (_int, [_vp, _u32]),
+    "mx4_pages_table": (_int, [_vp, _u32, _u32p, _u32p, _u32, _u32p]),
+    "mx4_pages_compact": (_int, [_vp, _u32p, _u32, _u32p]),
     "mx4_mfma_ceiling": (_int, [_vp, _int, _int, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double)]),
 }
 
@@ -121,6 +138,39 @@ def header_symbols() -> list[str]:
 class Op(ctypes.Structure):
     """mx4_op: one projection of a batch or recorded pass."""
     _fields_ = [("x", _vp), ("y", _vp), ("w", _vp), ("m", _u32), ("x_type", ctypes.c_int32)]
+
+
+def _addr(p) -> "int | None":
+    """A DeviceBuffer's address, or an address as it is (None: null)."""
+    return p.ptr if isinstance(p, DeviceBuffer) else p
+
+
+class KvCache(ctypes.Structure):
+    """mx4_kv_cache: a bf16 key/value cache [layers][pages][kv_heads][page_tokens][head_dim]
+    in caller-owned device memory (DeviceBuffers or addresses)."""
+    _fields_ = [("k", _vp), ("v", _vp), ("layer_stride", _u64), ("layers", _u32), ("pages", _u32), ("kv_heads", _u32),
+                ("page_tokens", _u32), ("head_dim", _u32)]
+
+    def __init__(self, k, v, layers: int, pages: int, kv_heads: int, page_tokens: int, head_dim: int, layer_stride: int = 0):
+        super().__init__(_addr(k), _addr(v), layer_stride, layers, pages, kv_heads, page_tokens, head_dim)
+        self._keep = (k, v)
+
+
+class Batch(ctypes.Structure):
+    """mx4_batch: the tokens of one call and where they live (uint32 device arrays)."""
+    _fields_ = [("seqs", _u32), ("tokens", _u32), ("max_tokens", _u32), ("table_stride", _u32), ("start", _vp),
+                ("cached", _vp), ("table", _vp)]
+
+    def __init__(self, seqs: int, tokens: int, max_tokens: int, start, cached, table, table_stride: int):
+        super().__init__(seqs, tokens, max_tokens, table_stride, _addr(start), _addr(cached), _addr(table))
+        self._keep = (start, cached, table)
+
+
+class Qkv(ctypes.Structure):
+    """mx4_qkv: the rows mx4_qk_norm_rope reads."""
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp), ("q_stride", _u64), ("k_stride", _u64), ("v_stride", _u64),
+                ("q_norm", _vp), ("k_norm", _vp), ("rope", _vp), ("positions", _vp), ("rope_positions", _u32),
+                ("q_heads", _u32), ("type", ctypes.c_int32), ("eps", ctypes.c_float)]
 
 
 class Mx4Error(RuntimeError):
@@ -278,6 +328,10 @@ class Context:
 
     def synchronize(self) -> None:
         check(lib().mx4_synchronize(self.handle))
+
+    def set_stream(self, stream: "int | None") -> None:
+        """Enqueue on a caller's hipStream_t (STREAM_LEGACY: the default stream; None: the context's own)."""
+        check(lib().mx4_set_stream(self.handle, stream))
 
     # weights
     def upload_weight(self, packed: np.ndarray, scales: np.ndarray, rows: int, cols: int) -> Weight:
@@ -468,6 +522,36 @@ class Context:
         check(lib().mx4_decode_table(self.handle, mode, out.ptr))
         return out.download(np.float32).reshape(256, 16)
 
+    # a step over a paged cache (device arguments: DeviceBuffers or addresses)
+    def rope_table(self, positions: int, head_dim: int, theta: float, out) -> None:
+        """Rows of head_dim floats: cosines, then sines, of position * theta^(-2 i / head_dim)."""
+        check(lib().mx4_rope_table(self.handle, positions, head_dim, theta, _addr(out)))
+
+    def qk_norm_rope(self, q, k, v, xtype: int, stride, q_heads: int, q_norm, k_norm, eps: float, rope, rope_positions: int,
+                     batch: Batch, cache: KvCache, layer: int, q_out, positions=None, q_out_stride: int = 0) -> None:
+        """Per-head norms, rotation and the cache write of a step's q, k, v rows (stride: elements
+        between tokens, one for all three or a (q, k, v) triple; 0: packed)."""
+        qs, ks, vs = stride if isinstance(stride, tuple) else (stride, stride, stride)
+        rows = Qkv(_addr(q), _addr(k), _addr(v), qs, ks, vs, _addr(q_norm), _addr(k_norm), _addr(rope), _addr(positions),
+                   rope_positions, q_heads, xtype, eps)
+        check(lib().mx4_qk_norm_rope(self.handle, ctypes.byref(rows), ctypes.byref(batch), ctypes.byref(cache), layer,
+                                     _addr(q_out), q_out_stride))
+
+    def attention(self, q, q_heads: int, batch: Batch, cache: KvCache, layer: int, out, tree=None, tree_words: int = 1,
+                  scale: float = 0.0, q_stride: int = 0, out_stride: int = 0) -> None:
+        """Attention of bf16 queries over the cache; tree: uint64 masks [tokens][tree_words], None: chains."""
+        check(lib().mx4_attention(self.handle, _addr(q), q_stride, q_heads, ctypes.byref(batch), ctypes.byref(cache), layer,
+                                  _addr(tree), tree_words, scale, _addr(out), out_stride))
+
+    def cache_copy_pages(self, cache: KvCache, pairs, count: int) -> None:
+        """Copy pages in every layer; pairs: uint32 device array [count][2] of (source, destination)."""
+        check(lib().mx4_cache_copy_pages(self.handle, ctypes.byref(cache), _addr(pairs), count))
+
+    def cache_keep(self, cache: KvCache, batch: Batch, kept, kept_count, max_kept: int) -> None:
+        """Move the kept new tokens (ascending, uint32 device array [seqs][max_kept]) to the front, in every layer."""
+        check(lib().mx4_cache_keep(self.handle, ctypes.byref(cache), ctypes.byref(batch), _addr(kept), _addr(kept_count),
+                                   max_kept))
+
     def compute_units(self) -> int:
         n = ctypes.c_int()
         check(lib().mx4_compute_units(self.handle, ctypes.byref(n)))
@@ -507,6 +591,68 @@ class Pass:
             self.release()
         except Exception:
             pass
+
+
+class Pages:
+    """Which pages of a cache belong to which sequence (mx4_pages, host only)."""
+
+    def __init__(self, pages: int, page_tokens: int):
+        h = _vp()
+        self.handle = None
+        check(lib().mx4_pages_create(pages, page_tokens, ctypes.byref(h)))
+        self.handle, self.pages = h.value, pages
+
+    def close(self) -> None:
+        if self.handle:
+            lib().mx4_pages_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def free_count(self) -> int:
+        n = _u32()
+        check(lib().mx4_pages_free_count(self.handle, ctypes.byref(n)))
+        return n.value
+
+    def open(self) -> int:
+        n = _u32()
+        check(lib().mx4_pages_open(self.handle, ctypes.byref(n)))
+        return n.value
+
+    def fork(self, seq: int) -> int:
+        n = _u32()
+        check(lib().mx4_pages_fork(self.handle, seq, ctypes.byref(n)))
+        return n.value
+
+    def write(self, seq: int, start: int, end: int) -> "list[tuple[int, int]]":
+        """Make positions start .. end - 1 writable; the page copies (source, destination) due first."""
+        pair, n = (_u32 * 2)(), _u32()
+        check(lib().mx4_pages_write(self.handle, seq, start, end, pair, ctypes.byref(n)))
+        return [(pair[0], pair[1])] if n.value else []
+
+    def trim(self, seq: int, tokens: int) -> None:
+        check(lib().mx4_pages_trim(self.handle, seq, tokens))
+
+    def close_sequence(self, seq: int) -> None:
+        check(lib().mx4_pages_close(self.handle, seq))
+
+    def table(self, seq: int) -> "tuple[int, list[int]]":
+        """A sequence's tokens and page numbers."""
+        tokens, n = _u32(), _u32()
+        check(lib().mx4_pages_table(self.handle, seq, ctypes.byref(tokens), None, 0, ctypes.byref(n)))
+        out = (_u32 * max(1, n.value))()
+        check(lib().mx4_pages_table(self.handle, seq, None, out, n.value, ctypes.byref(n)))
+        return tokens.value, list(out[:n.value])
+
+    def compact(self) -> "list[tuple[int, int]]":
+        """Renumber the pages in use to 0 .. n - 1; the page copies due."""
+        pairs, n = (_u32 * (2 * self.pages))(), _u32()
+        check(lib().mx4_pages_compact(self.handle, pairs, self.pages, ctypes.byref(n)))
+        return [(pairs[2 * i], pairs[2 * i + 1]) for i in range(n.value)]
 
 
 class Hip:
