@@ -1,0 +1,137 @@
+// attention_device.h -- what the attention kernels share: the running softmax's
+// constants, how a step is cut into chunks, and which keys a row sees.
+#pragma once
+
+#include "cache_device.h"
+
+namespace mx4 {
+
+constexpr float kNoMax = -3.4028234664e38f;  // below every score: 2^(s - kNoMax) is never taken, -inf - kNoMax = -inf
+// A row's maximum is raised only when a score passes it by this much: weights stay
+// below 2^8, their sums far inside f32, and most steps leave the accumulators alone.
+constexpr float kSlack = 8.0f;
+constexpr uint32_t kUnit = 128;  // keys: the grain in which a sequence is cut among workgroups
+
+// ------------------------------------------------------------- the split along the keys
+
+// How the step's work is cut. Every (row block, kv head) of a sequence has
+// ceil(units / cu) chunks of cu units; cu makes about `target` chunks a kv head of
+// the whole step, from the lengths in device memory. Chunks of cut rows leave
+// partial results in slots, joined by join_kernel. Only sequences of more than
+// `over` and at most `upto` rows a kv head take part. A sequence's last row block
+// comes first: in a prompt it has the most keys.
+struct Split {
+    uint32_t target, rows, over, upto;  // rows: of a row block
+};
+struct Chunk {
+    uint32_t s, blocks, block, chunk, chunks, slot, cu;  // slot: of the row block's first chunk, a kv head's numbering
+};
+
+struct Lengths {
+    uint32_t first, fresh, before, keys;
+};
+
+__device__ __forceinline__ bool not_finite(uint32_t pair) {  // either bf16 of a word
+    return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
+}
+
+__device__ __forceinline__ uint32_t finite_only(uint32_t pair) {  // zeros for what is not
+    if ((pair & 0x7f80u) == 0x7f80u) pair &= 0xffff0000u;
+    if ((pair & 0x7f800000u) == 0x7f800000u) pair &= 0xffffu;
+    return pair;
+}
+
+__device__ __forceinline__ Lengths lengths_of(const StepView& st, uint32_t s, uint32_t room) {
+    Lengths n;
+    tokens_of(st, s, n.first, n.fresh);
+    n.before = min(st.cached[s], room);
+    n.keys = min(n.before + n.fresh, room);
+    return n;
+}
+
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
+#pragma unroll
+    for (int off = 1; off < 64; off *= 2) v += __shfl_xor(v, off);
+    return v;
+}
+
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {  // inclusive
+    const uint32_t lane = threadIdx.x & 63;
+#pragma unroll
+    for (int off = 1; off < 64; off *= 2) {
+        const uint32_t o = __shfl_up(v, off);
+        v += lane >= (uint32_t)off ? o : 0;
+    }
+    return v;
+}
+
+// The chunk that is number `item` of its kv head, or (by_sequence) the first one of
+// sequence `item`'s last row block. False: there is none. Called by whole waves.
+__device__ __forceinline__ bool find_chunk(const StepView& st, uint32_t room, uint32_t group, const Split& split, uint32_t item,
+                                           bool by_sequence, Chunk& c) {
+    const uint32_t lane = threadIdx.x & 63;
+    auto shape = [&](uint32_t s, uint32_t& units, uint32_t& blocks) {
+        units = blocks = 0;
+        if (s >= st.seqs) return;
+        const Lengths n = lengths_of(st, s, room);
+        const uint32_t r = n.fresh * group;
+        if (n.fresh == 0 || r <= split.over || r > split.upto) return;
+        units = max((n.keys + kUnit - 1) / kUnit, 1u);
+        blocks = (r + split.rows - 1) / split.rows;
+    };
+    uint32_t total = 0;
+    for (uint32_t s0 = 0; s0 < st.seqs; s0 += 64) {
+        uint32_t units, blocks;
+        shape(s0 + lane, units, blocks);
+        total += wave_sum(units * blocks);
+    }
+    c.cu = max((total + split.target - 1) / split.target, 1u);
+    uint32_t items = 0, slots = 0;
+    for (uint32_t s0 = 0; s0 < st.seqs; s0 += 64) {
+        uint32_t units, blocks;
+        shape(s0 + lane, units, blocks);
+        const uint32_t chunks = (units + c.cu - 1) / c.cu, mine = chunks * blocks, cut = chunks > 1 ? mine : 0;
+        const uint32_t upto = items + wave_prefix(mine), slots_upto = slots + wave_prefix(cut);
+        const uint64_t hit = by_sequence ? (item - s0 < 64 ? 1ull << (item - s0) : 0ull) : __ballot(item < upto);
+        if (hit) {
+            const int at = __ffsll((unsigned long long)hit) - 1;
+            c.s = s0 + at;
+            c.chunks = __shfl(chunks, at);
+            const uint32_t in = by_sequence ? 0 : item - (__shfl(upto, at) - __shfl(mine, at));
+            if (c.chunks == 0) return false;
+            c.blocks = __shfl(blocks, at);
+            c.block = c.blocks - 1 - in / c.chunks;
+            c.chunk = in % c.chunks;
+            c.slot = __shfl(slots_upto, at) - __shfl(cut, at) + in / c.chunks * c.chunks;
+            return true;
+        }
+        items = __shfl(upto, 63);
+        slots = __shfl(slots_upto, 63);
+    }
+    return false;
+}
+
+// The keys that row (first + i) sees of the 32 from k0 on, one bit each.
+__device__ __forceinline__ uint32_t seen_window(const AttentionArgs& a, const Lengths& n, uint32_t i, uint32_t k0) {
+    const int64_t j0 = (int64_t)k0 - n.before;  // place among the new tokens
+    const int64_t most = (int64_t)n.keys - k0;  // keys that there are
+    const uint32_t there = most >= 32 ? ~0u : most <= 0 ? 0u : (1u << most) - 1;
+    if (!a.tree) {
+        const int64_t sees = (int64_t)i + 1 - j0;
+        return there & (sees >= 32 ? ~0u : sees <= 0 ? 0u : (1u << sees) - 1);
+    }
+    const uint64_t* row = a.tree + (uint64_t)(n.first + i) * a.tree_words;
+    auto word = [&](int64_t w) { return w < 0 ? ~0ull : w < a.tree_words ? row[w] : 0ull; };
+    const int64_t w = j0 >> 6;
+    const uint32_t shift = (uint32_t)(j0 & 63);
+    uint64_t bits = word(w) >> shift;
+    if (shift > 32) bits |= word(w + 1) << (64 - shift);
+    return there & (uint32_t)bits;
+}
+
+// attention.hip: adds up what the chunks of cut rows left in a.part.
+hipError_t launch_join(const AttentionArgs& a, const Split& split, uint32_t slot_rows);
+// attention_tiles.hip: sequences of more than `over` rows a kv head.
+hipError_t launch_attention_tiles(const AttentionArgs& a, uint32_t over, int cus);
+
+}  // namespace mx4
