@@ -24,7 +24,7 @@ struct Split {
     uint32_t target, rows, over, upto;  // rows: of a row block
 };
 struct Chunk {
-    uint32_t s, blocks, block, chunk, chunks, slot, cu;  // slot: of the row block's first chunk, a kv head's numbering
+    uint32_t s, block, chunk, chunks, slot, cu;  // slot: of the row block's first chunk, a kv head's numbering
 };
 
 struct Lengths {
@@ -65,12 +65,13 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {  // inclusive
     return v;
 }
 
-// The chunk that is number `item` of its kv head, or (by_sequence) the first one of
-// sequence `item`'s last row block. False: there is none. Called by whole waves.
+// The chunk that is number `item` of its kv head or, with `cut`, the first chunk of the
+// kv head's cut row block number `item`. False: there is none. Called by whole waves.
 __device__ __forceinline__ bool find_chunk(const StepView& st, uint32_t room, uint32_t group, const Split& split, uint32_t item,
-                                           bool by_sequence, Chunk& c) {
+                                           bool cut, Chunk& c) {
     const uint32_t lane = threadIdx.x & 63;
-    auto shape = [&](uint32_t s, uint32_t& units, uint32_t& blocks) {
+    uint32_t units = 0, blocks = 0, total = 0;
+    auto shape = [&](uint32_t s) {
         units = blocks = 0;
         if (s >= st.seqs) return;
         const Lengths n = lengths_of(st, s, room);
@@ -79,30 +80,26 @@ __device__ __forceinline__ bool find_chunk(const StepView& st, uint32_t room, ui
         units = max((n.keys + kUnit - 1) / kUnit, 1u);
         blocks = (r + split.rows - 1) / split.rows;
     };
-    uint32_t total = 0;
     for (uint32_t s0 = 0; s0 < st.seqs; s0 += 64) {
-        uint32_t units, blocks;
-        shape(s0 + lane, units, blocks);
+        shape(s0 + lane);
         total += wave_sum(units * blocks);
     }
     c.cu = max((total + split.target - 1) / split.target, 1u);
     uint32_t items = 0, slots = 0;
     for (uint32_t s0 = 0; s0 < st.seqs; s0 += 64) {
-        uint32_t units, blocks;
-        shape(s0 + lane, units, blocks);
-        const uint32_t chunks = (units + c.cu - 1) / c.cu, mine = chunks * blocks, cut = chunks > 1 ? mine : 0;
-        const uint32_t upto = items + wave_prefix(mine), slots_upto = slots + wave_prefix(cut);
-        const uint64_t hit = by_sequence ? (item - s0 < 64 ? 1ull << (item - s0) : 0ull) : __ballot(item < upto);
+        if (st.seqs > 64) shape(s0 + lane);
+        const uint32_t chunks = (units + c.cu - 1) / c.cu, in_slots = chunks > 1 ? chunks * blocks : 0;
+        const uint32_t mine = cut ? (chunks > 1 ? blocks : 0) : chunks * blocks;
+        const uint32_t upto = items + wave_prefix(mine), slots_upto = slots + wave_prefix(in_slots);
+        const uint64_t hit = __ballot(item < upto);
         if (hit) {
             const int at = __ffsll((unsigned long long)hit) - 1;
             c.s = s0 + at;
             c.chunks = __shfl(chunks, at);
-            const uint32_t in = by_sequence ? 0 : item - (__shfl(upto, at) - __shfl(mine, at));
-            if (c.chunks == 0) return false;
-            c.blocks = __shfl(blocks, at);
-            c.block = c.blocks - 1 - in / c.chunks;
-            c.chunk = in % c.chunks;
-            c.slot = __shfl(slots_upto, at) - __shfl(cut, at) + in / c.chunks * c.chunks;
+            const uint32_t in = item - (__shfl(upto, at) - __shfl(mine, at)), block = cut ? in : in / c.chunks;
+            c.block = __shfl(blocks, at) - 1 - block;
+            c.chunk = cut ? 0 : in % c.chunks;
+            c.slot = __shfl(slots_upto, at) - __shfl(in_slots, at) + block * c.chunks;
             return true;
         }
         items = __shfl(upto, 63);
@@ -129,8 +126,35 @@ __device__ __forceinline__ uint32_t seen_window(const AttentionArgs& a, const Le
     return there & (uint32_t)bits;
 }
 
-// attention.hip: adds up what the chunks of cut rows left in a.part.
-hipError_t launch_join(const AttentionArgs& a, const Split& split, uint32_t slot_rows);
+// New tokens' values that are not finite were left out of a row's products: the lane that
+// stored channel d of row r (to its slot in `part`, or the output) adds them to it if the
+// row sees the key (an infinite or NaN term is the same under any weight).
+__device__ __forceinline__ void add_to_stored(const AttentionArgs& a, const Chunk& c, const Lengths& n, uint32_t key, uint32_t kv,
+                                              uint32_t r, uint32_t row, uint32_t d, float* part) {
+    const uint32_t kvs = a.cache.kv_heads, group = a.q_heads / kvs, shift = a.cache.page_shift, dim = a.cache.head_dim;
+    const uint32_t page = min(a.step.table[(uint64_t)c.s * a.step.table_stride + (key >> shift)], a.cache.pages - 1);
+    const uint32_t bits = a.cache.v[((((uint64_t)page * kvs + kv) << shift) + (key & ((1u << shift) - 1))) * dim + d];
+    if ((bits & 0x7f80u) != 0x7f80u || !(seen_window(a, n, r / group, key) & 1)) return;
+    const float more = __uint_as_float(bits << 16);
+    if (c.chunks == 1) {
+        uint16_t* to = a.out + (uint64_t)(n.first + r / group) * a.out_stride + (uint64_t)(kv * group + r % group) * dim + d;
+        *to = __builtin_bit_cast(uint16_t, (__bf16)(__uint_as_float((uint32_t)*to << 16) + more));
+    } else {
+        part[row * dim + d] += more;
+    }
+}
+
+// Slots of slot_rows rows in the scratch: a cut row block has at least two chunks, so
+// `target` chunks a kv head leave at most that many and one more for every cut block.
+inline uint32_t split_target(const AttentionArgs& a, uint64_t wanted, uint64_t blocks, uint32_t slot_rows) {
+    const uint64_t slots = a.part_bytes / ((uint64_t)slot_rows * (a.cache.head_dim + 2) * 4) / a.cache.kv_heads;
+    const uint64_t most = slots > 2 * blocks ? slots - blocks : slots / 2;
+    const uint64_t target = wanted < most ? wanted : most;
+    return target < 1 ? 1 : (uint32_t)target;
+}
+// attention.hip: adds up what the chunks of cut rows left in a.part (blocks: row blocks
+// of a kv head, at most).
+hipError_t launch_join(const AttentionArgs& a, const Split& split, uint64_t blocks, uint32_t slot_rows);
 // attention_tiles.hip: sequences of more than `over` rows a kv head.
 hipError_t launch_attention_tiles(const AttentionArgs& a, uint32_t over, int cus);
 
