@@ -39,12 +39,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attention_rows_kernel(A
     const uint32_t kvs = a.cache.kv_heads, kv = blockIdx.y, group = a.q_heads / kvs, shift = a.cache.page_shift;
     const uint32_t room = table_room(a.step, shift);
     Chunk c;
-    if (!find_chunk(a.step, room, group, split, blockIdx.x, false, c)) return;
-    c.s = __builtin_amdgcn_readfirstlane(c.s);
-    const Lengths n = lengths_of(a.step, c.s, room);
+    Lengths n;
+    if (!find_chunk(a.step, room, group, split, blockIdx.x, false, c, n)) return;
     const uint32_t rows = n.fresh * group;
-    const uint32_t step0 = __builtin_amdgcn_readfirstlane(c.chunk * c.cu * (kUnit / 32));
-    const uint32_t step_end = __builtin_amdgcn_readfirstlane(min(step0 + c.cu * (kUnit / 32), (n.keys + 31) / 32));
+    const uint32_t step0 = c.chunk * c.cu * (kUnit / 32), step_end = min(step0 + c.cu * (kUnit / 32), (n.keys + 31) / 32);
     const uint32_t* table = a.step.table + (uint64_t)c.s * a.step.table_stride;
     const uint32_t in_page = (1u << shift) - 1;
 
@@ -219,57 +217,61 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attention_rows_kernel(A
             for (uint32_t x = 0; x < D / 16; ++x) add_to_stored(a, c, n, key, kv, row, row, d0 + x, part);
 }
 
-// A workgroup a cut row: its chunks' partial rows against their largest maximum, a
-// quarter of the chunks a wave, eight in flight; the order of the sums is fixed.
+// A workgroup takes rows of a cut row block, gridDim.z apart: the chunks' partial rows
+// against their largest maximum, a quarter of the chunks a wave, eight in flight; the
+// order of the sums is fixed.
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a, Split split, uint32_t slot_rows) {
     constexpr int E = D / 64, DEEP = 8;
-    __shared__ float sums[4][D], ls[4];
+    __shared__ float sums[2][4][D], ls[2][4];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t kvs = a.cache.kv_heads, kv = blockIdx.y, group = a.q_heads / kvs, row = blockIdx.z;
-    const uint32_t room = table_room(a.step, a.cache.page_shift);
+    const uint32_t kvs = a.cache.kv_heads, kv = blockIdx.y, group = a.q_heads / kvs;
     Chunk c;
-    if (!find_chunk(a.step, room, group, split, blockIdx.x, true, c)) return;
-    const Lengths n = lengths_of(a.step, c.s, room);
-    const uint32_t r = c.block * split.rows + row;
-    if (r >= n.fresh * group) return;
+    Lengths n;
+    if (!find_chunk(a.step, table_room(a.step, a.cache.page_shift), group, split, blockIdx.x, true, c, n)) return;
+    const uint32_t row0 = c.block * split.rows, rows = min(split.rows, n.fresh * group - row0);
     const uint64_t stride = (uint64_t)kvs * slot_rows * (D + 2);
-    const float* part = a.part + ((uint64_t)c.slot * kvs + kv) * slot_rows * (D + 2);
-    const float* stats = part + slot_rows * D + 2 * row;
-    part += row * D + lane * E;
-    float top = kNoMax;
-    for (uint32_t i = lane; i < c.chunks; i += 64) top = fmaxf(top, stats[i * stride]);
+    const float* slot = a.part + ((uint64_t)c.slot * kvs + kv) * slot_rows * (D + 2);
+    uint32_t side = 0;
+    for (uint32_t row = blockIdx.z; row < rows; row += gridDim.z, side ^= 1) {
+        const float* stats = slot + slot_rows * D + 2 * row;
+        const float* part = slot + row * D + lane * E;
+        float top = kNoMax;
+        for (uint32_t i = lane; i < c.chunks; i += 64) top = fmaxf(top, stats[i * stride]);
 #pragma unroll
-    for (int off = 1; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off));
-    float o[E] = {}, l = 0.0f;
-    for (uint32_t i0 = wave; i0 < c.chunks; i0 += 4 * DEEP) {
-        float x[DEEP][E], w[DEEP], add[DEEP];
+        for (int off = 1; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off));
+        float o[E] = {}, l = 0.0f;
+        for (uint32_t i0 = wave; i0 < c.chunks; i0 += 4 * DEEP) {
+            float x[DEEP][E], w[DEEP], add[DEEP];
 #pragma unroll
-        for (int u = 0; u < DEEP; ++u) {
-            const uint32_t at = min(i0 + 4 * u, c.chunks - 1);
-            w[u] = stats[at * stride];
-            add[u] = stats[at * stride + 1];
+            for (int u = 0; u < DEEP; ++u) {
+                const uint32_t at = min(i0 + 4 * u, c.chunks - 1);
+                w[u] = stats[at * stride];
+                add[u] = stats[at * stride + 1];
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[u][e] = part[at * stride + e];
+                for (int e = 0; e < E; ++e) x[u][e] = part[at * stride + e];
+            }
+#pragma unroll
+            for (int u = 0; u < DEEP; ++u) {
+                if (i0 + 4 * u >= c.chunks) break;
+                const float by = __builtin_amdgcn_exp2f(w[u] - top);
+                l = __builtin_fmaf(by, add[u], l);
+#pragma unroll
+                for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(by, x[u][e], o[e]);
+            }
         }
 #pragma unroll
-        for (int u = 0; u < DEEP; ++u) {
-            if (i0 + 4 * u >= c.chunks) break;
-            const float by = __builtin_amdgcn_exp2f(w[u] - top);
-            l = __builtin_fmaf(by, add[u], l);
-#pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(by, x[u][e], o[e]);
+        for (int e = 0; e < E; ++e) sums[side][wave][lane * E + e] = o[e];
+        if (lane == 0) ls[side][wave] = l;
+        __syncthreads();  // (two sides: a wave may be one row ahead of the readers)
+        if (tid < D) {
+            const float total = (ls[side][0] + ls[side][1]) + (ls[side][2] + ls[side][3]);
+            const float sum = (sums[side][0][tid] + sums[side][1][tid]) + (sums[side][2][tid] + sums[side][3][tid]);
+            const uint32_t r = row0 + row;
+            uint16_t* to = a.out + (uint64_t)(n.first + r / group) * a.out_stride + (uint64_t)(kv * group + r % group) * D;
+            to[tid] = __builtin_bit_cast(uint16_t, (__bf16)(total == 0.0f ? 0.0f : sum / total));
         }
     }
-#pragma unroll
-    for (int e = 0; e < E; ++e) sums[wave][lane * E + e] = o[e];
-    if (lane == 0) ls[wave] = l;
-    __syncthreads();
-    if (tid >= D) return;
-    l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
-    const float sum = (sums[0][tid] + sums[1][tid]) + (sums[2][tid] + sums[3][tid]);
-    uint16_t* to = a.out + (uint64_t)(n.first + r / group) * a.out_stride + (uint64_t)(kv * group + r % group) * D;
-    to[tid] = __builtin_bit_cast(uint16_t, (__bf16)(l == 0.0f ? 0.0f : sum / l));
 }
 
 template <int D>
@@ -280,12 +282,17 @@ hipError_t launch_rows(const AttentionArgs& a, uint32_t upto, int cus) {
     return launch_join(a, split, a.step.seqs, slot_rows);
 }
 
+constexpr uint32_t kJoins = 2048;
+
 }  // namespace
 
 hipError_t launch_join(const AttentionArgs& a, const Split& split, uint64_t blocks, uint32_t slot_rows) {
     // (a table of one unit's pages holds no sequence that could be cut)
     if (split.target > 1 && (uint64_t)a.step.table_stride << a.cache.page_shift > kUnit) {
-        const dim3 grid((uint32_t)(blocks < split.target ? blocks : split.target), a.cache.kv_heads, slot_rows);
+        const uint32_t cut = (uint32_t)(blocks < split.target ? blocks : split.target), kv = a.cache.kv_heads;
+        // a row a workgroup, but not more than kJoins workgroups: each has to find its row block first
+        const uint32_t z = kJoins / (cut * kv) < 1 ? 1 : kJoins / (cut * kv) > slot_rows ? slot_rows : kJoins / (cut * kv);
+        const dim3 grid(cut, kv, z);
         if (a.cache.head_dim == 64) join_kernel<64><<<grid, dim3(256), 0, a.stream>>>(a, split, slot_rows);
         if (a.cache.head_dim == 128) join_kernel<128><<<grid, dim3(256), 0, a.stream>>>(a, split, slot_rows);
         if (a.cache.head_dim == 256) join_kernel<256><<<grid, dim3(256), 0, a.stream>>>(a, split, slot_rows);

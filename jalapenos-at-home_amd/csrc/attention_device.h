@@ -49,61 +49,63 @@ __device__ __forceinline__ Lengths lengths_of(const StepView& st, uint32_t s, ui
     return n;
 }
 
-__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) v += __shfl_xor(v, off);
+// Inclusive sums over a wave's lanes.
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {
+#define MX4_STEP(ctrl, rows) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xf, false)
+    MX4_STEP(0x111, 0xf);  // row_shr 1, 2, 4, 8: within 16 lanes
+    MX4_STEP(0x112, 0xf);
+    MX4_STEP(0x114, 0xf);
+    MX4_STEP(0x118, 0xf);
+    MX4_STEP(0x142, 0xa);  // the last lane of rows 0 and 2 to rows 1 and 3
+    MX4_STEP(0x143, 0xc);  // that of row 1 to rows 2 and 3
+#undef MX4_STEP
     return v;
 }
 
-__device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {  // inclusive
-    const uint32_t lane = threadIdx.x & 63;
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) {
-        const uint32_t o = __shfl_up(v, off);
-        v += lane >= (uint32_t)off ? o : 0;
-    }
-    return v;
-}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, uint32_t lane) { return __builtin_amdgcn_readlane(v, lane); }
 
 // The chunk that is number `item` of its kv head or, with `cut`, the first chunk of the
-// kv head's cut row block number `item`. False: there is none. Called by whole waves.
+// kv head's cut row block number `item`, and its sequence's lengths. False: there is
+// none. Called by whole waves; everything it gives is the same in all lanes.
 __device__ __forceinline__ bool find_chunk(const StepView& st, uint32_t room, uint32_t group, const Split& split, uint32_t item,
-                                           bool cut, Chunk& c) {
+                                           bool cut, Chunk& c, Lengths& n) {
     const uint32_t lane = threadIdx.x & 63;
+    Lengths mine{};
     uint32_t units = 0, blocks = 0, total = 0;
     auto shape = [&](uint32_t s) {
         units = blocks = 0;
         if (s >= st.seqs) return;
-        const Lengths n = lengths_of(st, s, room);
-        const uint32_t r = n.fresh * group;
-        if (n.fresh == 0 || r <= split.over || r > split.upto) return;
-        units = max((n.keys + kUnit - 1) / kUnit, 1u);
+        mine = lengths_of(st, s, room);
+        const uint32_t r = mine.fresh * group;
+        if (mine.fresh == 0 || r <= split.over || r > split.upto) return;
+        units = max((mine.keys + kUnit - 1) / kUnit, 1u);
         blocks = (r + split.rows - 1) / split.rows;
     };
     for (uint32_t s0 = 0; s0 < st.seqs; s0 += 64) {
         shape(s0 + lane);
-        total += wave_sum(units * blocks);
+        total += lane_of(wave_prefix(units * blocks), 63);
     }
     c.cu = max((total + split.target - 1) / split.target, 1u);
     uint32_t items = 0, slots = 0;
     for (uint32_t s0 = 0; s0 < st.seqs; s0 += 64) {
         if (st.seqs > 64) shape(s0 + lane);
         const uint32_t chunks = (units + c.cu - 1) / c.cu, in_slots = chunks > 1 ? chunks * blocks : 0;
-        const uint32_t mine = cut ? (chunks > 1 ? blocks : 0) : chunks * blocks;
-        const uint32_t upto = items + wave_prefix(mine), slots_upto = slots + wave_prefix(in_slots);
+        const uint32_t count = cut ? (chunks > 1 ? blocks : 0) : chunks * blocks;
+        const uint32_t upto = items + wave_prefix(count), slots_upto = slots + wave_prefix(in_slots);
         const uint64_t hit = __ballot(item < upto);
         if (hit) {
-            const int at = __ffsll((unsigned long long)hit) - 1;
+            const uint32_t at = __ffsll((unsigned long long)hit) - 1;
             c.s = s0 + at;
-            c.chunks = __shfl(chunks, at);
-            const uint32_t in = item - (__shfl(upto, at) - __shfl(mine, at)), block = cut ? in : in / c.chunks;
-            c.block = __shfl(blocks, at) - 1 - block;
-            c.chunk = cut ? 0 : in % c.chunks;
-            c.slot = __shfl(slots_upto, at) - __shfl(in_slots, at) + block * c.chunks;
+            c.chunks = lane_of(chunks, at);
+            const uint32_t in = item - (lane_of(upto, at) - lane_of(count, at)), block = cut ? in : in / c.chunks;
+            c.block = lane_of(blocks, at) - 1 - block;
+            c.chunk = cut ? 0 : in - block * c.chunks;
+            c.slot = lane_of(slots_upto, at) - lane_of(in_slots, at) + block * c.chunks;
+            n = {lane_of(mine.first, at), lane_of(mine.fresh, at), lane_of(mine.before, at), lane_of(mine.keys, at)};
             return true;
         }
-        items = __shfl(upto, 63);
-        slots = __shfl(slots_upto, 63);
+        items = lane_of(upto, 63);
+        slots = lane_of(slots_upto, 63);
     }
     return false;
 }

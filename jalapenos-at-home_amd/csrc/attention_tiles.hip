@@ -150,17 +150,15 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
     const uint32_t kvs = a.cache.kv_heads, kv = blockIdx.x % kvs, group = a.q_heads / kvs, shift = a.cache.page_shift;
     const uint32_t room = table_room(a.step, shift);
     Chunk c;
-    if (!find_chunk(a.step, room, group, split, blockIdx.x / kvs, false, c)) return;
-    c.s = __builtin_amdgcn_readfirstlane(c.s);
-    const Lengths n = lengths_of(a.step, c.s, room);
+    Lengths n;
+    if (!find_chunk(a.step, room, group, split, blockIdx.x / kvs, false, c, n)) return;
     const uint32_t row0 = c.block * 128, all_rows = n.fresh * group;
     // chains: the keys that the block's last row sees; and how far all rows of the block see
     const uint32_t last_row = min(row0 + 128, all_rows) - 1;
     const uint32_t end_key = a.tree ? n.keys : min(n.keys, n.before + last_row / group + 1);
     const uint32_t clear = a.tree ? n.before : min(n.keys, n.before + row0 / group + 1);
-    const uint32_t tile0 = __builtin_amdgcn_readfirstlane(c.chunk * c.cu * (kUnit / kTile));
-    const uint32_t tile_end =
-        __builtin_amdgcn_readfirstlane(min(tile0 + c.cu * (kUnit / kTile), (end_key + kTile - 1) / kTile));
+    const uint32_t tile0 = c.chunk * c.cu * (kUnit / kTile);
+    const uint32_t tile_end = min(tile0 + c.cu * (kUnit / kTile), (end_key + kTile - 1) / kTile);
     Stage<D> st;
     st.k = a.cache.k;
     st.v = a.cache.v;
