@@ -16,6 +16,8 @@ namespace mx4 {
 
 namespace {
 
+typedef float f32x4_near __attribute__((ext_vector_type(4), aligned(8)));  // (a slot's rows follow pairs of floats)
+
 // ------------------------------------------------------------- few rows a sequence
 
 // A workgroup's four waves take the chunk's steps of 32 keys in turn, each with all 16
@@ -217,14 +219,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attention_rows_kernel(A
             for (uint32_t x = 0; x < D / 16; ++x) add_to_stored(a, c, n, key, kv, row, row, d0 + x, part);
 }
 
-// A workgroup takes rows of a cut row block, gridDim.z apart: the chunks' partial rows
-// against their largest maximum, a quarter of the chunks a wave, eight in flight; the
-// order of the sums is fixed.
+// A wave takes rows of a cut row block, 4 gridDim.z apart: the chunks' partial rows
+// against their largest maximum. A row is D / 4 lanes of four channels, so a wave has
+// 256 / D chunks side by side and eight such sets in flight; the order of the sums is
+// fixed.
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a, Split split, uint32_t slot_rows) {
-    constexpr int E = D / 64, DEEP = 8;
-    __shared__ float sums[2][4][D], ls[2][4];
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr uint32_t SIDE = 256 / D, DEEP = 8;
+    const uint32_t lane = threadIdx.x & 63, part_of = lane / (D / 4), d = lane % (D / 4) * 4;
     const uint32_t kvs = a.cache.kv_heads, kv = blockIdx.y, group = a.q_heads / kvs;
     Chunk c;
     Lengths n;
@@ -232,44 +234,53 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a, Split split,
     const uint32_t row0 = c.block * split.rows, rows = min(split.rows, n.fresh * group - row0);
     const uint64_t stride = (uint64_t)kvs * slot_rows * (D + 2);
     const float* slot = a.part + ((uint64_t)c.slot * kvs + kv) * slot_rows * (D + 2);
-    uint32_t side = 0;
-    for (uint32_t row = blockIdx.z; row < rows; row += gridDim.z, side ^= 1) {
+    for (uint32_t row = blockIdx.z * 4 + (threadIdx.x >> 6); row < rows; row += gridDim.z * 4) {
         const float* stats = slot + slot_rows * D + 2 * row;
-        const float* part = slot + row * D + lane * E;
+        const float* part = slot + row * D + d;
         float top = kNoMax;
         for (uint32_t i = lane; i < c.chunks; i += 64) top = fmaxf(top, stats[i * stride]);
+        f32x4 x[DEEP], o = {0, 0, 0, 0};
+        float l = 0.0f;
+        for (uint32_t w0 = 0; w0 < c.chunks; w0 += 64) {
+            const uint32_t left = min(c.chunks - w0, 64u);
+            const float* mine = stats + (w0 + min(lane, left - 1)) * stride;
+            const float mine_top = mine[0], mine_l = mine[1];
+            float weight = 0.0f;
+            for (uint32_t i0 = 0; i0 < left; i0 += SIDE * DEEP) {
 #pragma unroll
-        for (int off = 1; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off));
-        float o[E] = {}, l = 0.0f;
-        for (uint32_t i0 = wave; i0 < c.chunks; i0 += 4 * DEEP) {
-            float x[DEEP][E], w[DEEP], add[DEEP];
+                for (uint32_t u = 0; u < DEEP; ++u)
+                    x[u] = *reinterpret_cast<const f32x4_near*>(part + (w0 + min(i0 + u * SIDE + part_of, left - 1)) * stride);
+                if (i0 == 0) {
+                    if (w0 == 0)
 #pragma unroll
-            for (int u = 0; u < DEEP; ++u) {
-                const uint32_t at = min(i0 + 4 * u, c.chunks - 1);
-                w[u] = stats[at * stride];
-                add[u] = stats[at * stride + 1];
+                        for (int off = 1; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off));
+                    weight = lane < left ? __builtin_amdgcn_exp2f(mine_top - top) : 0.0f;
+                    l += lane < left ? weight * mine_l : 0.0f;
+                }
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[u][e] = part[at * stride + e];
-            }
+                for (uint32_t u = 0; u < DEEP; ++u) {
+                    const uint32_t at = i0 + u * SIDE + part_of;
+                    const float by = __shfl(weight, at & 63);
+                    if (at < left)
 #pragma unroll
-            for (int u = 0; u < DEEP; ++u) {
-                if (i0 + 4 * u >= c.chunks) break;
-                const float by = __builtin_amdgcn_exp2f(w[u] - top);
-                l = __builtin_fmaf(by, add[u], l);
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[e] = __builtin_fmaf(by, x[u][e], o[e]);
+                        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(by, x[u][e], o[e]);
+                }
             }
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e) sums[side][wave][lane * E + e] = o[e];
-        if (lane == 0) ls[side][wave] = l;
-        __syncthreads();  // (two sides: a wave may be one row ahead of the readers)
-        if (tid < D) {
-            const float total = (ls[side][0] + ls[side][1]) + (ls[side][2] + ls[side][3]);
-            const float sum = (sums[side][0][tid] + sums[side][1][tid]) + (sums[side][2][tid] + sums[side][3][tid]);
+        for (uint32_t off = D / 4; off < 64; off *= 2)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], off);
+#pragma unroll
+        for (int off = 1; off < 64; off *= 2) l += __shfl_xor(l, off);
+        const float by = l == 0.0f ? 0.0f : 1.0f / l;
+        if (part_of == 0) {
             const uint32_t r = row0 + row;
-            uint16_t* to = a.out + (uint64_t)(n.first + r / group) * a.out_stride + (uint64_t)(kv * group + r % group) * D;
-            to[tid] = __builtin_bit_cast(uint16_t, (__bf16)(total == 0.0f ? 0.0f : sum / total));
+            __bf16 b[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b[e] = (__bf16)(o[e] * by);
+            *reinterpret_cast<uint2*>(a.out + (uint64_t)(n.first + r / group) * a.out_stride + (uint64_t)(kv * group + r % group) * D + d) =
+                __builtin_bit_cast(uint2, b);
         }
     }
 }
@@ -290,8 +301,8 @@ hipError_t launch_join(const AttentionArgs& a, const Split& split, uint64_t bloc
     // (a table of one unit's pages holds no sequence that could be cut)
     if (split.target > 1 && (uint64_t)a.step.table_stride << a.cache.page_shift > kUnit) {
         const uint32_t cut = (uint32_t)(blocks < split.target ? blocks : split.target), kv = a.cache.kv_heads;
-        // a row a workgroup, but not more than kJoins workgroups: each has to find its row block first
-        const uint32_t z = kJoins / (cut * kv) < 1 ? 1 : kJoins / (cut * kv) > slot_rows ? slot_rows : kJoins / (cut * kv);
+        // a row a wave, but not more than kJoins workgroups: each has to find its row block first
+        const uint32_t most = kJoins / (cut * kv), whole = (slot_rows + 3) / 4, z = most < 1 ? 1 : most > whole ? whole : most;
         const dim3 grid(cut, kv, z);
         if (a.cache.head_dim == 64) join_kernel<64><<<grid, dim3(256), 0, a.stream>>>(a, split, slot_rows);
         if (a.cache.head_dim == 128) join_kernel<128><<<grid, dim3(256), 0, a.stream>>>(a, split, slot_rows);
@@ -307,8 +318,10 @@ constexpr uint32_t kFewRows = 16;
 hipError_t launch_attention(const AttentionArgs& a, int cus) {
     const uint64_t rows = (uint64_t)a.step.max_tokens * (a.q_heads / a.cache.kv_heads);
     const bool many = rows > kFewRows;
-    // (a step whose sequences all have max_tokens has none of the short kind)
-    if (!many || (uint64_t)a.step.seqs * a.step.max_tokens != a.step.tokens) {
+    // A step whose sequences all have max_tokens has none of the short kind. A mixed one of few
+    // sequences goes to the tiles as a whole: two launches less (9 us for 12 trees and for
+    // chunks beside decoding users) against 11 us for 32 decodes of 100 .. 8000 keys.
+    if (!many || (a.step.seqs > 16 && (uint64_t)a.step.seqs * a.step.max_tokens != a.step.tokens)) {
         const uint32_t most = many ? kFewRows : (uint32_t)rows;
         hipError_t e = hipSuccess;
         if (a.cache.head_dim == 64) e = launch_rows<64>(a, most, cus);
@@ -316,7 +329,8 @@ hipError_t launch_attention(const AttentionArgs& a, int cus) {
         if (a.cache.head_dim == 256) e = launch_rows<256>(a, most, cus);
         if (e != hipSuccess || !many) return e;
     }
-    return launch_attention_tiles(a, kFewRows, cus);
+    const bool all = a.step.seqs <= 16;
+    return launch_attention_tiles(a, all ? 0 : kFewRows, cus);
 }
 
 }  // namespace mx4

@@ -172,6 +172,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
     st.lane = lane;
 
     const uint32_t my_row = row0 + wave * 32 + n32, token = my_row < all_rows ? my_row / group : kNoRow;
+    const bool active = row0 + wave * 32 < all_rows;  // a wave without rows only helps with the loads
     bf16x8 q[KK];
     {
         const uint16_t* from = a.q + (uint64_t)(n.first + my_row / group) * a.q_stride + (uint64_t)(kv * group + my_row % group) * D + h * 8;
@@ -217,11 +218,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
                 if (tile + 2 < tile_end) wait_vm<4 * Stage<D>::LOADS>();
                 else wait_vm<0>();
                 lds_barrier();
+                if (active)
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk) {
-                    const bf16x8 kf = *reinterpret_cast<const bf16x8*>(&kbuf[0][kread[kk]]);
-                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[kk], kk ? s : f32x16{}, 0, 0, 0);
-                }
+                    for (int kk = 0; kk < KK; ++kk) {
+                        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(&kbuf[0][kread[kk]]);
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[kk], kk ? s : f32x16{}, 0, 0, 0);
+                    }
             }
             // the next tile is there, for every wave; the slot of the one before is free
             if (tile + 2 < tile_end) wait_vm<2 * Stage<D>::LOADS>();
@@ -245,6 +247,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
                 }
                 lds_barrier();
             }
+            if (!active) continue;
             s16x4 vf[MT][4];  // channels 32 m + .., rows 8 u + 4 h + ..
 #pragma unroll
             for (int m = 0; m < MT; ++m)
