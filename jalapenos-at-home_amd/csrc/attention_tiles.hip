@@ -85,6 +85,24 @@ __device__ __forceinline__ void finish(const AttentionArgs& a, const Chunk& c, c
         for (uint32_t e = 0; e < D / 2; ++e) add_to_stored(a, c, n, key, kv, r, row, e / 4 * 8 + h * 4 + e % 4, part);
 }
 
+// Direct-to-LDS load of 16 bytes a lane from `base` + offset (lane l's to `dst` + 16 l), which
+// returns nothing to a register. In assembly, because the compiler lets every transposing
+// read wait for all such loads that it knows of, the ones just issued too; here the waits are
+// wait_vm's. (What it waits for itself can only come later for it: the counter is in order.)
+__device__ __forceinline__ void load_to_lds(const uint16_t* base, uint32_t bytes, uint32_t offset, uint16_t* dst) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const uint64_t at = (uint64_t)base;
+    const u32x4 r = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, bytes, 0x00020000u};
+    const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t*)dst;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(to), "v"(offset), "s"(r)
+                 : "memory", "m0");
+#else
+    (void)base; (void)bytes; (void)offset; (void)dst;
+#endif
+}
+
 // A workgroup's way from the paged cache to the tiles, straight to LDS: D / 64 loads of
 // 1 KiB a wave, tile and side. A load's rows are neighbours of one 16-key group, so its
 // page is the wave's; the order of the pieces is made by the lanes' addresses.
@@ -94,16 +112,18 @@ struct Stage {
     const uint16_t *k, *v;
     const uint32_t* table;
     uint32_t table_last, page_last, kvs, kv, shift, wave, lane;
-    uint32_t pages, pages_next, pages_at;  // lane i: page of 16-key group 2 pages_at + i, and of the 64 groups after
-    uint32_t koff[LOADS], voff[LOADS];     // bytes from a group's first row
+    // lane i: page of 16-key half 2 pages_at + i; the table's entry for the 64 halves after (bounded
+    // when it is taken over, not before: that would wait for it)
+    uint32_t pages, entries_next, pages_at;
+    uint32_t koff[LOADS], voff[LOADS];     // bytes from a half's first row
 
     __device__ __forceinline__ uint32_t look_up(uint32_t tile) const {
-        return min(table[min((tile * 2 + lane) << 4 >> shift, table_last)], page_last);
+        return table[min((tile * 2 + lane) << 4 >> shift, table_last)];
     }
     __device__ __forceinline__ void begin(uint32_t tile) {
         pages_at = tile;
-        pages = look_up(tile);
-        pages_next = look_up(tile + 32);
+        pages = min(look_up(tile), page_last);
+        entries_next = look_up(tile + 32);
 #pragma unroll
         for (uint32_t i = 0; i < LOADS; ++i) {
             const uint32_t key = (wave * LOADS + i) * LOAD_ROWS + lane / ROW_LANES, piece = lane % ROW_LANES;
@@ -114,17 +134,17 @@ struct Stage {
     __device__ __forceinline__ void issue(uint32_t tile, uint16_t* kbuf, uint16_t* vbuf) {
         if (tile - pages_at == 32) {
             pages_at = tile;
-            pages = pages_next;
-            pages_next = look_up(tile + 32);
+            pages = min(entries_next, page_last);
+            entries_next = look_up(tile + 32);
         }
 #pragma unroll
         for (uint32_t i = 0; i < LOADS; ++i) {
-            const uint32_t load = wave * LOADS + i, group = load * LOAD_ROWS / 16;
-            const uint32_t page = __builtin_amdgcn_readlane(pages, (tile - pages_at) * 2 + group);
+            const uint32_t load = wave * LOADS + i, half = load * LOAD_ROWS / 16;
+            const uint32_t page = __builtin_amdgcn_readlane(pages, (tile - pages_at) * 2 + half);
             const uint64_t at =
-                ((((uint64_t)page * kvs + kv) << shift) + ((tile * kTile + group * 16) & ((1u << shift) - 1))) * D;
-            load_lds16(rsrc(k + at, 16 * D * 2), (lds_ptr)(kbuf + load * 512), koff[i]);
-            load_lds16(rsrc(v + at, 16 * D * 2), (lds_ptr)(vbuf + load * 512), voff[i]);
+                ((((uint64_t)page * kvs + kv) << shift) + ((tile * kTile + half * 16) & ((1u << shift) - 1))) * D;
+            load_to_lds(k + at, 16 * D * 2, koff[i], kbuf + load * 512);
+            load_to_lds(v + at, 16 * D * 2, voff[i], vbuf + load * 512);
         }
     }
 };
@@ -172,6 +192,13 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
     st.lane = lane;
 
     const uint32_t my_row = row0 + wave * 32 + n32, token = my_row < all_rows ? my_row / group : kNoRow;
+    auto fill = [&] {
+        st.begin(tile0);
+#pragma unroll
+        for (uint32_t i = 0; i < kRing - 1; ++i)
+            if (tile0 + i < tile_end) st.issue(tile0 + i, kbuf[i], vbuf[i]);
+    };
+    if (tile0 < tile_end) fill();
     const bool active = row0 + wave * 32 < all_rows;  // a wave without rows only helps with the loads
     bf16x8 q[KK];
     {
@@ -205,26 +232,20 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int x = 0; x < 16; ++x) acc[m][x] = 0.0f;
-        if (tile0 < tile_end) {
-            st.begin(tile0);
-#pragma unroll
-            for (uint32_t i = 0; i < kRing - 1; ++i)
-                if (tile0 + i < tile_end) st.issue(tile0 + i, kbuf[i], vbuf[i]);
-        }
         f32x16 s;
+        // the first tiles and the queries; the builtin, so that the compiler knows of it and waits
+        // for no load to registers inside the loop, where that would be all those to LDS too
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+        lds_barrier();
+        if (tile0 < tile_end) {
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+                const bf16x8 kf = *reinterpret_cast<const bf16x8*>(&kbuf[0][kread[kk]]);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[kk], kk ? s : f32x16{}, 0, 0, 0);
+            }
+        }
         for (uint32_t tile = tile0; tile < tile_end; ++tile) {
             const uint32_t slot = (tile - tile0) % kRing, after = (slot + 1) % kRing;
-            if (tile == tile0) {
-                if (tile + 2 < tile_end) wait_vm<4 * Stage<D>::LOADS>();
-                else wait_vm<0>();
-                lds_barrier();
-                if (active)
-#pragma unroll
-                    for (int kk = 0; kk < KK; ++kk) {
-                        const bf16x8 kf = *reinterpret_cast<const bf16x8*>(&kbuf[0][kread[kk]]);
-                        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[kk], kk ? s : f32x16{}, 0, 0, 0);
-                    }
-            }
             // the next tile is there, for every wave; the slot of the one before is free
             if (tile + 2 < tile_end) wait_vm<2 * Stage<D>::LOADS>();
             else wait_vm<0>();
@@ -306,6 +327,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
         lds_barrier();
         if (!again) break;
         careful = true;
+        fill();
     }
     if (careful) {
         lds_barrier();
