@@ -9,8 +9,8 @@ namespace mx4 {
 namespace {
 
 constexpr uint32_t kTile = 32;  // keys of a tile
-constexpr uint32_t kRing = 4;   // tiles in LDS: two being read, two on their way
 constexpr uint32_t kNoRow = 0xffffffffu;
+constexpr float kMostSum = 256.0f;  // 2^kSlack
 
 // A tile is 32 rows of D values, as they are in the cache, but for the order of a row's
 // 16-byte pieces. Keys are read as whole pieces, 16 rows at one piece a time: the
@@ -103,19 +103,20 @@ __device__ __forceinline__ void load_to_lds(const uint16_t* base, uint32_t bytes
 #endif
 }
 
-// A workgroup's way from the paged cache to the tiles, straight to LDS: D / 64 loads of
-// 1 KiB a wave, tile and side. A load's rows are neighbours of one 16-key group, so its
-// page is the wave's; the order of the pieces is made by the lanes' addresses.
+// A workgroup's way from the paged cache to the tiles, straight to LDS, 1 KiB a load: a
+// tile's keys, then its values, in runs of LOADS a wave. A load's rows are neighbours of one
+// 16-key half, so its page is the wave's; the order of the pieces is made by the lanes'
+// addresses.
 template <int D>
 struct Stage {
-    static constexpr uint32_t LOADS = D / 64, ROW_LANES = D / 8, LOAD_ROWS = 64 / ROW_LANES;
+    static constexpr uint32_t SIDE = D / 16, LOADS = 2 * SIDE / 4, ROW_LANES = D / 8, LOAD_ROWS = 64 / ROW_LANES;
     const uint16_t *k, *v;
     const uint32_t* table;
     uint32_t table_last, page_last, kvs, kv, shift, wave, lane;
     // lane i: page of 16-key half 2 pages_at + i; the table's entry for the 64 halves after (bounded
     // when it is taken over, not before: that would wait for it)
     uint32_t pages, entries_next, pages_at;
-    uint32_t koff[LOADS], voff[LOADS];     // bytes from a half's first row
+    uint32_t offset[LOADS];  // bytes from a half's first row
 
     __device__ __forceinline__ uint32_t look_up(uint32_t tile) const {
         return table[min((tile * 2 + lane) << 4 >> shift, table_last)];
@@ -126,34 +127,40 @@ struct Stage {
         entries_next = look_up(tile + 32);
 #pragma unroll
         for (uint32_t i = 0; i < LOADS; ++i) {
-            const uint32_t key = (wave * LOADS + i) * LOAD_ROWS + lane / ROW_LANES, piece = lane % ROW_LANES;
-            koff[i] = ((key & 15) * D + (piece ^ k_swap<D>(key)) * 8) * 2;
-            voff[i] = ((key & 15) * D + (piece ^ v_swap<D>(key)) * 8) * 2;
+            const uint32_t load = wave * LOADS + i, key = load % SIDE * LOAD_ROWS + lane / ROW_LANES;
+            const uint32_t swap = load < SIDE ? k_swap<D>(key) : v_swap<D>(key);
+            offset[i] = ((key & 15) * D + (lane % ROW_LANES ^ swap) * 8) * 2;
         }
     }
-    __device__ __forceinline__ void issue(uint32_t tile, uint16_t* kbuf, uint16_t* vbuf) {
+    // Tiles in turn: before the loads of one.
+    __device__ __forceinline__ void next(uint32_t tile) {
         if (tile - pages_at == 32) {
             pages_at = tile;
             pages = min(entries_next, page_last);
             entries_next = look_up(tile + 32);
         }
-#pragma unroll
-        for (uint32_t i = 0; i < LOADS; ++i) {
-            const uint32_t load = wave * LOADS + i, half = load * LOAD_ROWS / 16;
-            const uint32_t page = __builtin_amdgcn_readlane(pages, (tile - pages_at) * 2 + half);
-            const uint64_t at =
-                ((((uint64_t)page * kvs + kv) << shift) + ((tile * kTile + half * 16) & ((1u << shift) - 1))) * D;
-            load_to_lds(k + at, 16 * D * 2, koff[i], kbuf + load * 512);
-            load_to_lds(v + at, 16 * D * 2, voff[i], vbuf + load * 512);
-        }
+    }
+    // (there: else nothing is read, and zeros go to LDS -- the count of the loads stays)
+    __device__ __forceinline__ void issue(uint32_t tile, uint32_t i, bool there, uint16_t* kbuf, uint16_t* vbuf) {
+        const uint32_t load = wave * LOADS + i, half = load % SIDE * LOAD_ROWS / 16;
+        const uint32_t page = __builtin_amdgcn_readlane(pages, (tile - pages_at) * 2 + half);
+        const uint64_t at =
+            ((((uint64_t)page * kvs + kv) << shift) + ((tile * kTile + half * 16) & ((1u << shift) - 1))) * D;
+        load_to_lds((load < SIDE ? k : v) + at, there ? 16 * D * 2 : 0, offset[i], (load < SIDE ? kbuf : vbuf) + load % SIDE * 512);
     }
 };
 
 // Four waves, each with 32 rows against the workgroup's keys, 32 at a time in LDS.
 // S^T = K Q^T in 32 x 32 x 16 products leaves lane (row n = lane % 32, half h) the scores
 // of keys 8 b + 4 h + i; packed in that order they are the operand P^T of O^T = V^T P^T.
-// A wave's step: values of tile j to registers, weights of tile j, keys of tile j + 1 to
-// registers, the products of both; the other wave of its SIMD fills the pauses.
+// A wave's step j is laid out by hand so that little waits: a product keeps the matrix
+// cores for 32 cycles, in which the wave does what stands behind it here: the reads of
+// tile j + 1's keys beside tile j's values, the loads of tile j + 4 and the reads of tile
+// j + 1's values beside the scores of tile j + 1. (Loads issued in a bunch after the barrier
+// took 580 of a step's 2000 cycles.)
+//
+// The maximum is not looked for: a row whose weights' sum passes 2^kSlack has to raise it,
+// and takes its weights again.
 //
 // A weight of zero times an infinite or NaN value would spread NaN to rows that do not
 // see its key. The products are first taken as they are; only if a result is not
@@ -162,8 +169,10 @@ struct Stage {
 template <int D>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(AttentionArgs a, Split split, uint32_t slot_rows) {
     constexpr int KK = D / 16, MT = D / 32;
-    __shared__ __align__(16) uint16_t kbuf[kRing][kTile * D];
-    __shared__ __align__(16) uint16_t vbuf[kRing][kTile * D];
+    constexpr uint32_t ROWS = 128, RING = 4;  // tiles in LDS: the one being read and three on their way
+    constexpr uint32_t LOADS = Stage<D>::LOADS;
+    __shared__ __align__(16) uint16_t kbuf[RING][kTile * D];
+    __shared__ __align__(16) uint16_t vbuf[RING][kTile * D];
     __shared__ uint32_t again;
     const uint32_t tid = threadIdx.x, lane = tid & 63, n32 = lane & 31, h = lane >> 5;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -172,9 +181,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
     Chunk c;
     Lengths n;
     if (!find_chunk(a.step, room, group, split, blockIdx.x / kvs, false, c, n)) return;
-    const uint32_t row0 = c.block * 128, all_rows = n.fresh * group;
+    const uint32_t row0 = c.block * ROWS, all_rows = n.fresh * group;
     // chains: the keys that the block's last row sees; and how far all rows of the block see
-    const uint32_t last_row = min(row0 + 128, all_rows) - 1;
+    const uint32_t last_row = min(row0 + ROWS, all_rows) - 1;
     const uint32_t end_key = a.tree ? n.keys : min(n.keys, n.before + last_row / group + 1);
     const uint32_t clear = a.tree ? n.before : min(n.keys, n.before + row0 / group + 1);
     const uint32_t tile0 = c.chunk * c.cu * (kUnit / kTile);
@@ -190,15 +199,16 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
     st.shift = shift;
     st.wave = wave;
     st.lane = lane;
-
-    const uint32_t my_row = row0 + wave * 32 + n32, token = my_row < all_rows ? my_row / group : kNoRow;
     auto fill = [&] {
         st.begin(tile0);
 #pragma unroll
-        for (uint32_t i = 0; i < kRing - 1; ++i)
-            if (tile0 + i < tile_end) st.issue(tile0 + i, kbuf[i], vbuf[i]);
+        for (uint32_t r = 0; r < RING; ++r)
+#pragma unroll
+            for (uint32_t i = 0; i < LOADS; ++i) st.issue(tile0 + r, i, tile0 + r < tile_end, kbuf[r], vbuf[r]);
     };
     if (tile0 < tile_end) fill();
+
+    const uint32_t my_row = row0 + wave * 32 + n32, token = my_row < all_rows ? my_row / group : kNoRow;
     const bool active = row0 + wave * 32 < all_rows;  // a wave without rows only helps with the loads
     bf16x8 q[KK];
     {
@@ -211,15 +221,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
         }
     }
     const float cs = a.scale * 1.44269504088896340736f;
-    // where the lane reads in a tile (elements): key n32's pieces 2 kk + h, and for channels
-    // 32 m + 16 (lane / 16 % 2) + .. of rows 4 h + lane % 16 / 4 (+ 8 u') the quarter-row piece
-    uint32_t kread[KK], vread[MT];
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) kread[kk] = n32 * D + ((kk * 2 + h) ^ k_swap<D>(n32)) * 8;
+    // Where the lane reads in a tile (elements): key n32's pieces 2 kk + h, and for channels
+    // 32 m + 16 (lane / 16 % 2) + .. of rows 4 h + lane % 16 / 4 (+ 8 u) the quarter-row piece.
+    // (kk and m stand in bits of their own, so they are xored on.)
     const uint32_t vrow = h * 4 + (lane & 15) / 4;
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-        vread[m] = vrow * D + ((m * 4 + (lane >> 4 & 1) * 2 + (lane & 3) / 2) ^ v_swap<D>(vrow)) * 8 + (lane & 1) * 4;
+    const uint32_t kread = n32 * D + (h ^ k_swap<D>(n32)) * 8;
+    const uint32_t vread = vrow * D + (((lane >> 4 & 1) * 2 + (lane & 3) / 2) ^ v_swap<D>(vrow)) * 8 + (lane & 1) * 4;
 
     f32x16 acc[MT];
     float top, l;
@@ -229,93 +236,125 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
         top = kNoMax;
         l = 0.0f;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < MT; ++m) acc[m] = f32x16{};
+        // values behind the last key become zeros, and (careful) so do those that are not finite;
+        // all threads, between two barriers
+        auto mend = [&](uint32_t tile, uint32_t slot) {
+            if (tile >= tile_end || tile * kTile + kTile <= (careful ? n.before : n.keys)) return;
+            for (uint32_t i = tid; i < kTile * D / 8; i += 256) {
+                u32x4 w = *reinterpret_cast<u32x4*>(&vbuf[slot][i * 8]);
+                const bool there = tile * kTile + i / (D / 8) < n.keys;
 #pragma unroll
-            for (int x = 0; x < 16; ++x) acc[m][x] = 0.0f;
-        f32x16 s;
+                for (int x = 0; x < 4; ++x) {
+                    w[x] = there ? w[x] : 0u;
+                    if (careful) {
+                        found |= not_finite(w[x]);
+                        w[x] = finite_only(w[x]);
+                    }
+                }
+                *reinterpret_cast<u32x4*>(&vbuf[slot][i * 8]) = w;
+            }
+            lds_barrier();
+        };
+        f32x16 s{};
+        s16x4 vf[MT][4];  // channels 32 m + .., rows 8 u + 4 h + ..
+        auto read_values = [&](uint32_t from, int r) { vf[r / 4][r % 4] = read_turned(&vbuf[0][(from ^ r / 4 * 32) + r % 4 * 8 * D]); };
         // the first tiles and the queries; the builtin, so that the compiler knows of it and waits
         // for no load to registers inside the loop, where that would be all those to LDS too
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
         lds_barrier();
         if (tile0 < tile_end) {
+            mend(tile0, 0);
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk) {
-                const bf16x8 kf = *reinterpret_cast<const bf16x8*>(&kbuf[0][kread[kk]]);
+                const bf16x8 kf = *reinterpret_cast<const bf16x8*>(&kbuf[0][kread ^ kk * 16]);
                 s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[kk], kk ? s : f32x16{}, 0, 0, 0);
             }
+#pragma unroll
+            for (int r = 0; r < 4 * MT; ++r) read_values(vread, r);
         }
-        for (uint32_t tile = tile0; tile < tile_end; ++tile) {
-            const uint32_t slot = (tile - tile0) % kRing, after = (slot + 1) % kRing;
-            // the next tile is there, for every wave; the slot of the one before is free
-            if (tile + 2 < tile_end) wait_vm<2 * Stage<D>::LOADS>();
-            else wait_vm<0>();
+        // The next tile has landed, for every wave, and this one's slot is free.
+        auto turn = [&](uint32_t tile) {
+            wait_vm<2 * LOADS>();
             lds_barrier();
-            if (tile + 3 < tile_end) st.issue(tile + 3, kbuf[(slot + 3) % kRing], vbuf[(slot + 3) % kRing]);
-            if (tile * kTile + kTile > (careful ? n.before : n.keys)) {
-                // (before any read of this tile's values, and after every load of them)
-                for (uint32_t i = tid; i < kTile * D / 8; i += 256) {
-                    u32x4 w = *reinterpret_cast<u32x4*>(&vbuf[slot][i * 8]);
-                    const bool there = tile * kTile + i / (D / 8) < n.keys;
+            mend(tile + 1, (tile + 1 - tile0) % RING);
+            st.next(tile + RING);
+        };
+        auto issue = [&](uint32_t tile, uint32_t i) {
+            const uint32_t slot = (tile - tile0) % RING;
+            st.issue(tile + RING, i, tile + RING < tile_end, kbuf[slot], vbuf[slot]);
+        };
+        if (!active)
+            for (uint32_t tile = tile0; tile < tile_end; ++tile) {
+                turn(tile);
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        w[x] = there ? w[x] : 0u;
-                        if (careful) {
-                            found |= not_finite(w[x]);
-                            w[x] = finite_only(w[x]);
-                        }
-                    }
-                    *reinterpret_cast<u32x4*>(&vbuf[slot][i * 8]) = w;
-                }
-                lds_barrier();
+                for (uint32_t i = 0; i < LOADS; ++i) issue(tile, i);
             }
-            if (!active) continue;
-            s16x4 vf[MT][4];  // channels 32 m + .., rows 8 u + 4 h + ..
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int u = 0; u < 4; ++u) vf[m][u] = read_turned(&vbuf[slot][vread[m] + u * 8 * D]);
-            __builtin_amdgcn_sched_barrier(0);
+        for (uint32_t tile = active ? tile0 : tile_end; tile < tile_end; ++tile) {
+            const uint32_t after = (tile + 1 - tile0) % RING;
+            turn(tile);
             if (tile * kTile + kTile > clear) {
                 const uint32_t seen = token != kNoRow ? seen_window(a, n, token, tile * kTile) : 0u;
 #pragma unroll
                 for (int x = 0; x < 16; ++x)
                     if (!(seen >> (x / 4 * 8 + h * 4 + x % 4) & 1)) s[x] = -INFINITY;
             }
-            float most = s[0];
+            bf16x8 p[2];  // rounded to bf16 for the products; their sum is of the rounded ones
+            float sum;
+            const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
+            auto weigh = [&](int x) {  // weights x and x + 1
+                bf16x2 w = {(__bf16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[x], cs, -top)),
+                            (__bf16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[x + 1], cs, -top))};
+                asm volatile("" : "+v"(w));  // made here, not where it is used
+                p[x / 8][x % 8] = w[0];
+                p[x / 8][x % 8 + 1] = w[1];
+                sum = __builtin_amdgcn_fdot2_f32_bf16(w, one, x ? sum : 0.0f, false);
+            };
+            auto add_values = [&](int u, int m) {
+                const uint2 lo = __builtin_bit_cast(uint2, vf[m][2 * u]), hi = __builtin_bit_cast(uint2, vf[m][2 * u + 1]);
+                const uint4 w = {lo.x, lo.y, hi.x, hi.y};
+                acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), p[u], acc[m], 0, 0, 0);
+            };
 #pragma unroll
-            for (int x = 1; x < 16; ++x) most = fmaxf(most, s[x]);
-            most *= cs;
-            if (__any(most > top + kSlack)) {
+            for (int x = 0; x < 16; x += 2) weigh(x);
+            if (__any(sum > kMostSum)) {
+                float most = s[0];
+#pragma unroll
+                for (int x = 1; x < 16; ++x) most = fmaxf(most, s[x]);
+                most *= cs;
                 most = fmaxf(most, __shfl_xor(most, 32));
                 const float now = fmaxf(top, most), keep = __builtin_amdgcn_exp2f(top - now);
                 top = now;
                 l *= keep;
 #pragma unroll
                 for (int m = 0; m < MT; ++m) acc[m] *= keep;
+#pragma unroll
+                for (int x = 0; x < 16; x += 2) weigh(x);
             }
-            bf16x8 p[2];
-#pragma unroll
-            for (int x = 0; x < 16; ++x) p[x / 8][x % 8] = (__bf16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[x], cs, -top));
-            const bf16x2 one = {(__bf16)1.0f, (__bf16)1.0f};
-#pragma unroll
-            for (int x = 0; x < 8; ++x)  // the sum of the rounded weights
-                l = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{p[x / 4][x % 4 * 2], p[x / 4][x % 4 * 2 + 1]}, one, l, false);
+            l += sum;
             __builtin_amdgcn_sched_barrier(0);
+            // (behind the last tile: scores of whatever the slot holds, which nothing uses)
+            const uint32_t from_k = kread + after * kTile * D, from_v = vread + after * kTile * D;
             bf16x8 kf[KK];
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) kf[kk] = *reinterpret_cast<const bf16x8*>(&kbuf[after][kread[kk]]);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int i = 0; i < 2 * MT; ++i) {
+                add_values(i / MT, i % MT);
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+                for (int kk = 0; kk < KK; ++kk)
+                    if (kk * 2 * MT / KK == i) kf[kk] = *reinterpret_cast<const bf16x8*>(&kbuf[0][from_k ^ kk * 16]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const uint4 w = {__builtin_bit_cast(uint2, vf[m][2 * u]).x, __builtin_bit_cast(uint2, vf[m][2 * u]).y,
-                                     __builtin_bit_cast(uint2, vf[m][2 * u + 1]).x, __builtin_bit_cast(uint2, vf[m][2 * u + 1]).y};
-                    acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, w), p[u], acc[m], 0, 0, 0);
-                }
-            // (behind the last tile: of whatever the slot holds, and unused)
+            for (int kk = 0; kk < KK; ++kk) {
+                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk], q[kk], kk ? s : f32x16{}, 0, 0, 0);
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kk], q[kk], kk ? s : f32x16{}, 0, 0, 0);
+                for (uint32_t i = 0; i < LOADS; ++i)
+                    if (i * KK / LOADS == (uint32_t)kk) issue(tile, i);
+#pragma unroll
+                for (int r = 0; r < 4 * MT; ++r)
+                    if (r * KK / (4 * MT) == kk) read_values(from_v, r);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         if (careful) break;
         bool odd = false;
