@@ -141,8 +141,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attention_rows_kernel(A
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (!(seen >> (half * 16 + g * 4 + e) & 1)) s[half][e] = -INFINITY;
-            // values of keys that are not there count as zeros; so do new tokens' values that are
-            // not finite, which the rows that see them get at the end
+            // values of keys that are not there count as zeros; so do those that are not finite,
+            // which the rows that see them get at the end
 #pragma unroll
             for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attention_rows_kernel(A
         }
     }
     if (bad)
-        for (uint32_t key = max(step0 * 32, n.before); key < min(step_end * 32, n.keys); ++key)
+        for (uint32_t key = max(step0 * 32, n.before & ~31u); key < min(step_end * 32, n.keys); ++key)  // the steps not whole
 #pragma unroll 1
             for (uint32_t x = 0; x < D / 16; ++x) add_to_stored(a, c, n, key, kv, row, row, d0 + x, part);
 }

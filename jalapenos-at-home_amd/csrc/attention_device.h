@@ -14,9 +14,11 @@ constexpr uint32_t kUnit = 128;  // keys: the grain in which a sequence is cut a
 
 // ------------------------------------------------------------- the split along the keys
 
+constexpr uint32_t kUncut = 1u << 24;  // units: 2^31 keys, more than a sequence has
+
 // How the step's work is cut. Every (row block, kv head) of a sequence has
 // ceil(units / cu) chunks of cu units; cu makes about `target` chunks a kv head of
-// the whole step, from the lengths in device memory. Chunks of cut rows leave
+// the whole step, from the lengths in device memory; a target of 1 cuts nothing. Chunks of cut rows leave
 // partial results in slots, joined by join_kernel. Only sequences of more than
 // `over` and at most `upto` rows a kv head take part. A sequence's last row block
 // comes first: in a prompt it has the most keys.
@@ -83,9 +85,9 @@ __device__ __forceinline__ bool find_chunk(const StepView& st, uint32_t room, ui
     };
     for (uint32_t s0 = 0; s0 < st.seqs; s0 += 64) {
         shape(s0 + lane);
-        total += lane_of(wave_prefix(units * blocks), 63);
+        if (split.target > 1) total += lane_of(wave_prefix(units * blocks), 63);
     }
-    c.cu = max((total + split.target - 1) / split.target, 1u);
+    c.cu = split.target > 1 ? max((total + split.target - 1) / split.target, 1u) : kUncut;
     uint32_t items = 0, slots = 0;
     for (uint32_t s0 = 0; s0 < st.seqs; s0 += 64) {
         if (st.seqs > 64) shape(s0 + lane);
@@ -128,7 +130,8 @@ __device__ __forceinline__ uint32_t seen_window(const AttentionArgs& a, const Le
     return there & (uint32_t)bits;
 }
 
-// New tokens' values that are not finite were left out of a row's products: the lane that
+// Values that are not finite were left out of a row's products, where not every row sees every
+// key: the lane that
 // stored channel d of row r (to its slot in `part`, or the output) adds them to it if the
 // row sees the key (an infinite or NaN term is the same under any weight).
 __device__ __forceinline__ void add_to_stored(const AttentionArgs& a, const Chunk& c, const Lengths& n, uint32_t key, uint32_t kv,
@@ -148,7 +151,10 @@ __device__ __forceinline__ void add_to_stored(const AttentionArgs& a, const Chun
 
 // Slots of slot_rows rows in the scratch: a cut row block has at least two chunks, so
 // `target` chunks a kv head leave at most that many and one more for every cut block.
+// (A step whose units may not be counted in 32 bits fills the device uncut.)
 inline uint32_t split_target(const AttentionArgs& a, uint64_t wanted, uint64_t blocks, uint32_t slot_rows) {
+    const uint64_t units = ((uint64_t)a.step.table_stride << a.cache.page_shift) / kUnit + 1;
+    if (units >> 32 || blocks * units >> 31) return 1;
     const uint64_t slots = a.part_bytes / ((uint64_t)slot_rows * (a.cache.head_dim + 2) * 4) / a.cache.kv_heads;
     const uint64_t most = slots > 2 * blocks ? slots - blocks : slots / 2;
     const uint64_t target = wanted < most ? wanted : most;

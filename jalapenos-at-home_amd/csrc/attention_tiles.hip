@@ -80,7 +80,7 @@ __device__ __forceinline__ void finish(const AttentionArgs& a, const Chunk& c, c
         }
     }
     if (!found) return;
-    for (uint32_t key = max(key0, n.before); key < key_end && token != kNoRow; ++key)
+    for (uint32_t key = max(key0, n.before & ~(kTile - 1)); key < key_end && token != kNoRow; ++key)
 #pragma unroll 1
         for (uint32_t e = 0; e < D / 2; ++e) add_to_stored(a, c, n, key, kv, r, row, e / 4 * 8 + h * 4 + e % 4, part);
 }
@@ -164,8 +164,8 @@ struct Stage {
 //
 // A weight of zero times an infinite or NaN value would spread NaN to rows that do not
 // see its key. The products are first taken as they are; only if a result is not
-// finite they are taken again with such new tokens' values left out (found), which the
-// rows that see them get at the end. What stands behind the last key never counts.
+// finite they are taken again with such values left out (found) in the tiles that hold new
+// tokens, and the rows that see them get them at the end. What stands behind the last key never counts.
 template <int D>
 __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(AttentionArgs a, Split split, uint32_t slot_rows) {
     constexpr int KK = D / 16, MT = D / 32;
@@ -366,6 +366,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
         lds_barrier();
         if (!again) break;
         careful = true;
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): nothing of the first pass is on its way to the slots
         fill();
     }
     if (careful) {

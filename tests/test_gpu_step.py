@@ -244,6 +244,75 @@ def test_attention_masked_places_have_no_part(mx4, ctx, new, cached, bad):
         assert np.all(np.isnan(got[hit]))
 
 
+@pytest.mark.parametrize("new,cached,hq,hk,d,page", [
+    # steps whose short and long sequences take different kernels
+    ([1, 40, 2, 90, 1, 0, 1, 33] + [1] * 13, [900, 3, 70, 0, 5, 8, 2000, 31] + list(range(13)), 8, 2, 128, 16),
+    ([30] + [1] * 20, [500] + [130] * 20, 12, 4, 64, 32), ([1] * 19 + [9, 70], [40] * 20 + [600], 8, 2, 256, 16),
+    # more than a wave's lanes: sequences that are cut, and a row's chunks
+    ([1, 2] * 40, [300, 0, 10, 1500] * 20, 4, 2, 64, 16), ([40, 30] * 36, [20, 200, 3] * 24, 2, 1, 64, 16),
+    ([1], [20000], 8, 1, 128, 16), ([40], [9000], 4, 1, 64, 16),
+])
+def test_attention_batches(mx4, ctx, new, cached, hq, hk, d, page):
+    rng = np.random.default_rng(hq * 1000 + d + sum(new) + sum(cached))
+    step = Step(mx4, ctx, rng, new, cached, hk, d, page).fill(rng)
+    got, q = attend(step, rng, hq)
+    near(got, *reference(step, q, hq, chain(step)))
+
+
+@pytest.mark.parametrize("new,cached,hq,hk,d,page", [(1, 70000, 64, 64, 64, 16), (2, 140003, 64, 32, 128, 16),
+                                                   (40, 9001, 64, 64, 64, 16), (70, 20000, 32, 32, 128, 64), (33, 40000, 16, 16, 256, 16)])
+def test_attention_long_way_of_one_workgroup(mx4, ctx, new, cached, hq, hk, d, page):
+    """Many heads and keys, so that a workgroup walks through many entries of the page table --
+    of few pages, each of which many entries name: a key's weight counts as often as it stands there."""
+    rng = np.random.default_rng(new + cached)
+    pages, entries, group = 37, -(-(new + cached) // page), hq // hk
+    kv = [to_bits(rng.standard_normal((pages, hk, page, d))) for _ in range(2)]
+    table = rng.integers(0, pages, entries).astype(np.uint32)
+    k, v = (ctx.to_device(x) for x in kv)
+    dev = [ctx.to_device(np.asarray(x, np.uint32)) for x in ([0, new], [cached], table)]
+    q = to_bits(rng.standard_normal((new, hq, d)))
+    out = ctx.buffer(q.nbytes)
+    ctx.attention(ctx.to_device(q), hq, mx4.Batch(1, new, new, *dev, entries), mx4.KvCache(k, v, 1, pages, hk, page, d), 0, out)
+    got = from_bits(out.download(np.uint16)).reshape(q.shape)
+    want, tol = np.zeros(q.shape), np.zeros(q.shape)
+    kf, vf = (from_bits(x).astype(np.float64).transpose(1, 0, 2, 3).reshape(hk, pages * page, d) for x in kv)
+    qf = from_bits(q).astype(np.float64)
+    for i in range(new):
+        at = np.arange(cached + i + 1)
+        times = np.bincount(table[at // page].astype(np.int64) * page + at % page, minlength=pages * page)
+        for h in range(hq):
+            x = kf[h // group] @ qf[i, h] * d ** -0.5
+            w = times * np.exp(x - x[times > 0].max())
+            w /= w.sum()
+            want[i, h] = w @ vf[h // group]
+            slip = 2 * (d + 4) * 2.0 ** -24 * (np.abs(kf[h // group]) @ np.abs(qf[i, h]) * d ** -0.5).max() + 2.0 ** -18
+            tol[i, h] = U * np.abs(want[i, h]) + (2 * U + 2 * slip) * 1.01 * (w @ np.abs(vf[h // group])) + 1e-30
+    near(got, want, tol)
+
+
+@pytest.mark.parametrize("new,cached", [([12], [20]), ([80], [3]), ([2], [40]), ([12, 100], [131, 94]), ([300], [1000])])
+@pytest.mark.parametrize("back", [1, 3])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_attention_cached_values_that_are_not_finite(mx4, ctx, new, cached, back, bad):
+    """Every row of the sequence sees the cached keys, also those that stand in a tile with new ones."""
+    rng = np.random.default_rng(sum(new) + back)
+    step = Step(mx4, ctx, rng, new, cached, 2, 128, 16).fill(rng)
+    where = step.at(0, cached[0] - back)[1, 60:62]
+    step.kv[1][0][where] = 0
+    step.up()
+    masks = random_tree(rng, step, 5)
+    sees = from_masks(step, masks.reshape(-1), 5)
+    _, q = attend(step, np.random.default_rng(8), 4, masks, 5)
+    want, tol = reference(step, q, 4, sees)
+    step.kv[1][0][where] = to_bits(np.float32(bad))
+    step.up()
+    got, _ = attend(step, np.random.default_rng(8), 4, masks, 5)
+    hit = np.zeros(got.shape, bool)
+    hit[:new[0], 2:, 60:62] = True
+    near(got[~hit], want[~hit], tol[~hit])
+    assert np.array_equal(got[hit], np.full(hit.sum(), bad, np.float32), equal_nan=True)
+
+
 @pytest.mark.parametrize("new,cached", [([1], [2000]), ([20], [333]), ([150], [0])])
 def test_attention_large_scores(mx4, ctx, new, cached):
     """Scores of thousands, and a maximum that grows with every key."""
