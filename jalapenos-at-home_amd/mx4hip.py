@@ -231,6 +231,10 @@ class DeviceBuffer:
         check(lib().mx4_malloc(ctx.handle, max(self.nbytes, 1), ctypes.byref(p)))
         self.ptr = p.value
 
+    @property
+    def _as_parameter_(self) -> "int | None":  # what ctypes passes
+        return self.ptr
+
     def upload(self, a: np.ndarray, offset: int = 0) -> "DeviceBuffer":
         a = np.ascontiguousarray(a)
         assert offset + a.nbytes <= self.nbytes
@@ -525,32 +529,34 @@ class Context:
     # a step over a paged cache (device arguments: DeviceBuffers or addresses)
     def rope_table(self, positions: int, head_dim: int, theta: float, out) -> None:
         """Rows of head_dim floats: cosines, then sines, of position * theta^(-2 i / head_dim)."""
-        check(lib().mx4_rope_table(self.handle, positions, head_dim, theta, _addr(out)))
+        check(lib().mx4_rope_table(self.handle, positions, head_dim, theta, out))
 
     def qk_norm_rope(self, q, k, v, xtype: int, stride, q_heads: int, q_norm, k_norm, eps: float, rope, rope_positions: int,
                      batch: Batch, cache: KvCache, layer: int, q_out, positions=None, q_out_stride: int = 0) -> None:
         """Per-head norms, rotation and the cache write of a step's q, k, v rows (stride: elements
         between tokens, one for all three or a (q, k, v) triple; 0: packed)."""
         qs, ks, vs = stride if isinstance(stride, tuple) else (stride, stride, stride)
-        rows = Qkv(_addr(q), _addr(k), _addr(v), qs, ks, vs, _addr(q_norm), _addr(k_norm), _addr(rope), _addr(positions),
-                   rope_positions, q_heads, xtype, eps)
+        try:
+            rows = Qkv(q, k, v, qs, ks, vs, q_norm, k_norm, rope, positions, rope_positions, q_heads, xtype, eps)
+        except TypeError:  # not all addresses
+            rows = Qkv(_addr(q), _addr(k), _addr(v), qs, ks, vs, _addr(q_norm), _addr(k_norm), _addr(rope), _addr(positions),
+                       rope_positions, q_heads, xtype, eps)
         check(lib().mx4_qk_norm_rope(self.handle, ctypes.byref(rows), ctypes.byref(batch), ctypes.byref(cache), layer,
-                                     _addr(q_out), q_out_stride))
+                                     q_out, q_out_stride))
 
     def attention(self, q, q_heads: int, batch: Batch, cache: KvCache, layer: int, out, tree=None, tree_words: int = 1,
                   scale: float = 0.0, q_stride: int = 0, out_stride: int = 0) -> None:
         """Attention of bf16 queries over the cache; tree: uint64 masks [tokens][tree_words], None: chains."""
-        check(lib().mx4_attention(self.handle, _addr(q), q_stride, q_heads, ctypes.byref(batch), ctypes.byref(cache), layer,
-                                  _addr(tree), tree_words, scale, _addr(out), out_stride))
+        check(lib().mx4_attention(self.handle, q, q_stride, q_heads, ctypes.byref(batch), ctypes.byref(cache), layer, tree,
+                                  tree_words, scale, out, out_stride))
 
     def cache_copy_pages(self, cache: KvCache, pairs, count: int) -> None:
         """Copy pages in every layer; pairs: uint32 device array [count][2] of (source, destination)."""
-        check(lib().mx4_cache_copy_pages(self.handle, ctypes.byref(cache), _addr(pairs), count))
+        check(lib().mx4_cache_copy_pages(self.handle, ctypes.byref(cache), pairs, count))
 
     def cache_keep(self, cache: KvCache, batch: Batch, kept, kept_count, max_kept: int) -> None:
         """Move the kept new tokens (ascending, uint32 device array [seqs][max_kept]) to the front, in every layer."""
-        check(lib().mx4_cache_keep(self.handle, ctypes.byref(cache), ctypes.byref(batch), _addr(kept), _addr(kept_count),
-                                   max_kept))
+        check(lib().mx4_cache_keep(self.handle, ctypes.byref(cache), ctypes.byref(batch), kept, kept_count, max_kept))
 
     def compute_units(self) -> int:
         n = ctypes.c_int()
