@@ -509,6 +509,52 @@ def test_keep(mx4, ctx, new, cached, kept, hk, d, page):
         assert np.array_equal(side, x)
 
 
+def test_a_recorded_step(mx4, ctx):
+    """Norms, rotation, attention, kept tokens and a page copy in one pass: each replay gives what the
+    calls give, with the lengths, lists and pairs that the device holds then."""
+    rng = np.random.default_rng(21)
+    hq, hk, d, page = 8, 2, 128, 16
+    step = Step(mx4, ctx, rng, [9, 30], [200, 31], hk, d, page, layers=2, layer=1).fill(rng)
+    rows = rng.standard_normal((step.tokens, (hq + 2 * hk) * d)).astype(np.float32)
+    x, norm, rope = ctx.to_device(rows), ctx.to_device(to_bits(rng.uniform(0.5, 2, d))), ctx.buffer(300 * d * 4)
+    ctx.rope_table(300, d, 1e6, rope)
+    q, out = ctx.buffer(step.tokens * hq * d * 2), ctx.buffer(step.tokens * hq * d * 2)
+    masks = ctx.to_device(random_tree(rng, step, 1, empty=0.0))
+    kept, counts = ctx.to_device(np.zeros((2, 6), np.uint32)), ctx.to_device(np.zeros(2, np.uint32))
+    pairs = ctx.to_device(np.zeros((1, 2), np.uint32))
+    width = rows.shape[1]
+
+    def run():
+        ctx.qk_norm_rope(x.ptr, x.ptr + hq * d * 4, x.ptr + (hq + hk) * d * 4, mx4.F32, width, hq, norm, norm, 1e-6, rope, 300,
+                         step.batch, step.cache, 1, q)
+        ctx.attention(q, hq, step.batch, step.cache, 1, out, masks)
+        ctx.cache_keep(step.cache, step.batch, kept, counts, 6)
+        ctx.cache_copy_pages(step.cache, pairs, 1)
+
+    def state(cached, lists, pair):
+        step.dev["cached"].upload(np.array(cached, np.uint32))
+        kept.upload(np.array([list(x) + [0] * (6 - len(x)) for x in lists], np.uint32))
+        counts.upload(np.array([len(x) for x in lists], np.uint32))
+        pairs.upload(np.array([pair], np.uint32))
+        for buf, x in zip((step.k, step.v), step.kv):
+            buf.upload(x)
+        out.upload(np.zeros(out.nbytes, np.uint8))
+
+    recorded = ctx.record(run)
+    for cached, lists, pair in [([200, 31], [[0, 3, 8], [1, 2, 20, 29]], (2, 5)), ([3, 0], [[], [0]], (1, 0)),
+                                ([150, 17], [[8], [4, 5, 6, 7, 8, 9]], (4, 4)), ([200, 31], [[0, 3, 8], [1, 2, 20, 29]], (2, 5))]:
+        state(cached, lists, pair)
+        recorded.launch()
+        ctx.synchronize()
+        replay = [out.download(np.uint16)] + step.down()
+        state(cached, lists, pair)
+        run()
+        ctx.synchronize()
+        for a, b in zip(replay, [out.download(np.uint16)] + step.down()):
+            assert np.array_equal(a, b)
+    recorded.release()
+
+
 def test_offsets_past_32_bits(mx4, ctx):
     """Pages whose elements start past 2^32 of the cache."""
     rng = np.random.default_rng(12)
@@ -630,3 +676,17 @@ def test_refusals(mx4, ctx):
         assert 1 <= e.value.status <= 4 or e.value.status == 9, i
     attention(b=batch(tokens=0, max_tokens=0))  # nothing to do
     rope(b=batch(tokens=0, max_tokens=0))
+
+
+def test_example_decodes_the_same_tokens_by_trees(mx4):
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parent.parent / "examples" / "tree_decode.py"
+    spec = importlib.util.spec_from_file_location("tree_decode", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    plain, trees, steps, free = example.main()
+    assert trees == plain and len(set(plain)) > 8
+    assert steps < len(plain)
+    both = -(-(45 + len(plain)) // example.PAGE)
+    assert free == example.PAGES - (2 * both - 45 // example.PAGE)
