@@ -325,9 +325,9 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a, Split split,
 }
 
 template <int D>
-hipError_t launch_rows(const AttentionArgs& a, uint32_t upto, int cus) {
-    const uint32_t kv = a.cache.kv_heads, rows = a.step.max_tokens * (a.q_heads / kv), slot_rows = rows < upto ? rows : upto;
-    const Split split{split_target(a, 4ull * cus / kv, a.step.seqs, slot_rows), 16, 0, upto};
+hipError_t launch_rows(const AttentionArgs& a, int cus) {
+    const uint32_t kv = a.cache.kv_heads, slot_rows = a.step.max_tokens * (a.q_heads / kv);
+    const Split split{split_target(a, 4ull * cus / kv, a.step.seqs, slot_rows), 16};
     attention_rows_kernel<D><<<dim3(split.target + a.step.seqs, kv), dim3(256), 0, a.stream>>>(a, split, slot_rows);
     return launch_join(a, split, a.step.seqs, slot_rows);
 }
@@ -351,26 +351,17 @@ hipError_t launch_join(const AttentionArgs& a, const Split& split, uint64_t bloc
     return hipGetLastError();
 }
 
-// Sequences of up to 16 rows a kv head (one product's) read their keys to registers;
-// the others share them in LDS.
+// Steps of up to 16 rows a sequence and kv head (one product's) read their keys to registers,
+// the others share them in LDS, single tokens beside longer runs too. Of 32 sequences of 100 ..
+// 8000 keys at 32 / 8 heads of 128, 8 and 16 rows: 68 and 58 us against 75 and 57 in LDS; with
+// one of them a prompt's 200 tokens, 78 us in a launch for either kind against 59.
 constexpr uint32_t kFewRows = 16;
 
 hipError_t launch_attention(const AttentionArgs& a, int cus) {
-    const uint64_t rows = (uint64_t)a.step.max_tokens * (a.q_heads / a.cache.kv_heads);
-    const bool many = rows > kFewRows;
-    // A step whose sequences all have max_tokens has none of the short kind. A mixed one of few
-    // sequences goes to the tiles as a whole: two launches less (9 us for 12 trees and for
-    // chunks beside decoding users) against 11 us for 32 decodes of 100 .. 8000 keys.
-    if (!many || (a.step.seqs > 16 && (uint64_t)a.step.seqs * a.step.max_tokens != a.step.tokens)) {
-        const uint32_t most = many ? kFewRows : (uint32_t)rows;
-        hipError_t e = hipSuccess;
-        if (a.cache.head_dim == 64) e = launch_rows<64>(a, most, cus);
-        if (a.cache.head_dim == 128) e = launch_rows<128>(a, most, cus);
-        if (a.cache.head_dim == 256) e = launch_rows<256>(a, most, cus);
-        if (e != hipSuccess || !many) return e;
-    }
-    const bool all = a.step.seqs <= 16;
-    return launch_attention_tiles(a, all ? 0 : kFewRows, cus);
+    if ((uint64_t)a.step.max_tokens * (a.q_heads / a.cache.kv_heads) > kFewRows) return launch_attention_tiles(a, cus);
+    if (a.cache.head_dim == 64) return launch_rows<64>(a, cus);
+    if (a.cache.head_dim == 128) return launch_rows<128>(a, cus);
+    return launch_rows<256>(a, cus);
 }
 
 }  // namespace mx4

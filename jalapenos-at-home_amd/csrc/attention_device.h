@@ -19,11 +19,10 @@ constexpr uint32_t kUncut = 1u << 24;  // units: 2^31 keys, more than a sequence
 // How the step's work is cut. Every (row block, kv head) of a sequence has
 // ceil(units / cu) chunks of cu units; cu makes about `target` chunks a kv head of
 // the whole step, from the lengths in device memory; a target of 1 cuts nothing. Chunks of cut rows leave
-// partial results in slots, joined by join_kernel. Only sequences of more than
-// `over` and at most `upto` rows a kv head take part. A sequence's last row block
+// partial results in slots, joined by join_kernel. A sequence's last row block
 // comes first: in a prompt it has the most keys.
 struct Split {
-    uint32_t target, rows, over, upto;  // rows: of a row block
+    uint32_t target, rows;  // rows: of a row block
 };
 struct Chunk {
     uint32_t s, block, chunk, chunks, slot, cu;  // slot: of the row block's first chunk, a kv head's numbering
@@ -78,10 +77,9 @@ __device__ __forceinline__ bool find_chunk(const StepView& st, uint32_t room, ui
         units = blocks = 0;
         if (s >= st.seqs) return;
         mine = lengths_of(st, s, room);
-        const uint32_t r = mine.fresh * group;
-        if (mine.fresh == 0 || r <= split.over || r > split.upto) return;
+        if (mine.fresh == 0) return;
         units = max((mine.keys + kUnit - 1) / kUnit, 1u);
-        blocks = (r + split.rows - 1) / split.rows;
+        blocks = (mine.fresh * group + split.rows - 1) / split.rows;
     };
     for (uint32_t s0 = 0; s0 < st.seqs; s0 += 64) {
         shape(s0 + lane);
@@ -163,7 +161,7 @@ inline uint32_t split_target(const AttentionArgs& a, uint64_t wanted, uint64_t b
 // attention.hip: adds up what the chunks of cut rows left in a.part (blocks: row blocks
 // of a kv head, at most).
 hipError_t launch_join(const AttentionArgs& a, const Split& split, uint64_t blocks, uint32_t slot_rows);
-// attention_tiles.hip: sequences of more than `over` rows a kv head.
-hipError_t launch_attention_tiles(const AttentionArgs& a, uint32_t over, int cus);
+// attention_tiles.hip: steps of many rows a kv head.
+hipError_t launch_attention_tiles(const AttentionArgs& a, int cus);
 
 }  // namespace mx4

@@ -381,26 +381,29 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
 }
 
 template <int D>
-hipError_t launch_tiles(const AttentionArgs& a, uint32_t over, int cus) {
+hipError_t launch_tiles(const AttentionArgs& a, int cus) {
     constexpr uint32_t ROWS = 128;
     const uint32_t group = a.q_heads / a.cache.kv_heads, kv = a.cache.kv_heads;
     const uint64_t rows = (uint64_t)a.step.max_tokens * group;
     // row blocks of a kv head: the tokens' whole ones, and a partial one a sequence
     const uint64_t whole = (uint64_t)a.step.tokens * group / ROWS, blocks = whole + a.step.seqs;
     const uint32_t slot_rows = rows < ROWS ? (uint32_t)rows : ROWS;
-    // enough row blocks to fill the CUs several times over need no cutting
-    const uint64_t wanted = whole * kv >= 4ull * cus ? 1 : 2ull * cus / kv;
-    const Split split{split_target(a, wanted, blocks, slot_rows), ROWS, over, 0xffffffffu};
+    // Two workgroups a CU, as many as are there at a time: 12 trees of 9 .. 32 tokens take 35 us,
+    // with one a CU 41; 25 tokens behind 39000 take 49 and 47 (half the partial rows), with three
+    // 61. One sequence of as many row blocks would not be cut, which saves the join's launch.
+    uint32_t target = split_target(a, 2ull * cus / kv, blocks, slot_rows);
+    if (a.step.seqs == 1 && whole >= target) target = 1;
+    const Split split{target, ROWS};
     attention_tiles_kernel<D><<<dim3((uint32_t)((split.target + blocks) * kv)), dim3(256), 0, a.stream>>>(a, split, slot_rows);
     return launch_join(a, split, blocks, slot_rows);
 }
 
 }  // namespace
 
-hipError_t launch_attention_tiles(const AttentionArgs& a, uint32_t over, int cus) {
-    if (a.cache.head_dim == 64) return launch_tiles<64>(a, over, cus);
-    if (a.cache.head_dim == 128) return launch_tiles<128>(a, over, cus);
-    return launch_tiles<256>(a, over, cus);
+hipError_t launch_attention_tiles(const AttentionArgs& a, int cus) {
+    if (a.cache.head_dim == 64) return launch_tiles<64>(a, cus);
+    if (a.cache.head_dim == 128) return launch_tiles<128>(a, cus);
+    return launch_tiles<256>(a, cus);
 }
 
 }  // namespace mx4

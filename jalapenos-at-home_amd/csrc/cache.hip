@@ -125,9 +125,9 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeArgs a) {
 
 hipError_t launch_qk_norm_rope(const RopeArgs& a, int cus) {
     const uint32_t heads = a.q_heads + 2 * a.cache.kv_heads, per_block = 4 * 64 / (a.cache.head_dim / 8);
-    uint32_t y = (heads + per_block - 1) / per_block;
-    if (a.step.tokens >= 4u * cus) y = 1;
-    const dim3 grid(a.step.tokens, y);
+    // Few tokens have their heads side by side, of many each is one workgroup's: one token of 16 / 8
+    // heads takes 3.0 us against 3.9, 512 of 32 / 8 heads take 8.1 against 7.9.
+    const dim3 grid(a.step.tokens, a.step.tokens < (uint32_t)cus ? (heads + per_block - 1) / per_block : 1);
 #define MX4_ROPE(D)                                                                               \
     if (a.cache.head_dim == D) {                                                                  \
         if (a.x_bf16) qk_norm_rope_kernel<D, true><<<grid, dim3(256), 0, a.stream>>>(a);          \
