@@ -150,13 +150,22 @@ __device__ __forceinline__ void add_to_stored(const AttentionArgs& a, const Chun
 // Slots of slot_rows rows in the scratch: a cut row block has at least two chunks, so
 // `target` chunks a kv head leave at most that many and one more for every cut block.
 // (A step whose units may not be counted in 32 bits fills the device uncut.)
+inline uint64_t most_units(const AttentionArgs& a) {  // that a sequence of this page table can have
+    const uint64_t room = (uint64_t)a.step.table_stride << a.cache.page_shift;
+    return room < kUnit ? 1 : (room + kUnit - 1) / kUnit;
+}
 inline uint32_t split_target(const AttentionArgs& a, uint64_t wanted, uint64_t blocks, uint32_t slot_rows) {
-    const uint64_t units = ((uint64_t)a.step.table_stride << a.cache.page_shift) / kUnit + 1;
+    const uint64_t units = most_units(a);
     if (units >> 32 || blocks * units >> 31) return 1;
     const uint64_t slots = a.part_bytes / ((uint64_t)slot_rows * (a.cache.head_dim + 2) * 4) / a.cache.kv_heads;
     const uint64_t most = slots > 2 * blocks ? slots - blocks : slots / 2;
     const uint64_t target = wanted < most ? wanted : most;
     return target < 1 ? 1 : (uint32_t)target;
+}
+// Workgroups a kv head: a chunk each, of `target` and one more a row block at most.
+inline uint32_t most_chunks(const AttentionArgs& a, uint32_t target, uint64_t blocks) {
+    const uint64_t all = blocks * most_units(a);  // (target > 1: below 2^31)
+    return (uint32_t)(target > 1 && all < target + blocks ? all : target + blocks);
 }
 // attention.hip: adds up what the chunks of cut rows left in a.part (blocks: row blocks
 // of a kv head, at most).

@@ -394,7 +394,7 @@ hipError_t launch_tiles(const AttentionArgs& a, int cus) {
     uint32_t target = split_target(a, 2ull * cus / kv, blocks, slot_rows);
     if (a.step.seqs == 1 && whole >= target) target = 1;
     const Split split{target, ROWS};
-    attention_tiles_kernel<D><<<dim3((uint32_t)((split.target + blocks) * kv)), dim3(256), 0, a.stream>>>(a, split, slot_rows);
+    attention_tiles_kernel<D><<<dim3(most_chunks(a, split.target, blocks) * kv), dim3(256), 0, a.stream>>>(a, split, slot_rows);
     return launch_join(a, split, blocks, slot_rows);
 }
 

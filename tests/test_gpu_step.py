@@ -251,6 +251,8 @@ def test_attention_masked_places_have_no_part(mx4, ctx, new, cached, bad):
     # more than a wave's lanes: sequences that are cut, and a row's chunks
     ([1, 2] * 40, [300, 0, 10, 1500] * 20, 4, 2, 64, 16), ([40, 30] * 36, [20, 200, 3] * 24, 2, 1, 64, 16),
     ([1], [20000], 8, 1, 128, 16), ([40], [9000], 4, 1, 64, 16),
+    # one sequence of more row blocks than the device takes at a time, and beside a longer one
+    ([600], [0], 128, 128, 64, 16), ([600, 1], [0, 3000], 64, 64, 64, 16),
 ])
 def test_attention_batches(mx4, ctx, new, cached, hq, hk, d, page):
     rng = np.random.default_rng(hq * 1000 + d + sum(new) + sum(cached))
