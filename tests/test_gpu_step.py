@@ -490,7 +490,8 @@ def test_copy_pages(mx4, ctx, layers, hk, d, page, pages, count):
 @pytest.mark.parametrize("new,cached,kept,hk,d,page", [
     ([1], [0], [[0]], 1, 64, 16), ([9], [10], [[0, 2, 3, 8]], 8, 128, 16), ([9], [14], [[1, 2, 3, 4, 5, 6, 7, 8]], 2, 64, 16),
     ([0, 5, 64, 3], [7, 16, 31, 0], [[], [0, 4], list(range(0, 64, 2)), [2]], 3, 128, 16),
-    ([200], [5], [list(range(1, 200))], 2, 256, 32), ([70, 70], [0, 90], [list(range(30, 70)), [69]], 5, 128, 64)])
+    ([200], [5], [list(range(1, 200))], 2, 256, 32), ([70, 70], [0, 90], [list(range(30, 70)), [69]], 5, 128, 64),
+    ([4, 3] * 50, list(range(100)), [[0, 2, 3], [1]] * 50, 5, 64, 16)])
 def test_keep(mx4, ctx, new, cached, kept, hk, d, page):
     rng = np.random.default_rng(sum(new))
     step = Step(mx4, ctx, rng, new, cached, hk, d, page, layers=3, pad_layer=8).fill(rng)
