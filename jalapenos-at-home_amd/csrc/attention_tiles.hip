@@ -162,6 +162,13 @@ struct Stage {
 // The maximum is not looked for: a row whose weights' sum passes 2^kSlack has to raise it,
 // and takes its weights again.
 //
+// Bound: a prompt's 8001 tokens (32 / 8 heads of 128, 524 GFLOP behind the mask) take 515 us, 1018
+// TFLOP/s; a large library product makes 1239, and as there the clock falls under the load (to
+// 1.6 GHz with the matrix cores half busy). Two workgroups share a CU, which fills what the one
+// leaves; with one the prompt takes 800 us, with 64 rows a wave (one wave a SIMD) 571. Trees of 9
+// .. 32 tokens (91 MB of cache) are bound by its bytes, 27 us of 35 with the join; chunks of
+// prompts (1 .. 900 tokens) by the last row block's way through its keys, 1.1 us a tile.
+//
 // A weight of zero times an infinite or NaN value would spread NaN to rows that do not
 // see its key. The products are first taken as they are; only if a result is not
 // finite they are taken again with such values left out (found) in the tiles that hold new

@@ -261,7 +261,7 @@ struct RopeArgs {
 };
 hipError_t launch_qk_norm_rope(const RopeArgs& a, int cus);
 // pairs [count][2]: page pairs[2 i] of every layer to page pairs[2 i + 1]
-hipError_t launch_copy_pages(const CacheView& c, const uint32_t* pairs, uint32_t count, int cus, hipStream_t s);
+hipError_t launch_copy_pages(const CacheView& c, const uint32_t* pairs, uint32_t count, hipStream_t s);
 // kept [seqs][max_kept], ascending: new token kept[s][j] of sequence s becomes its new token j
 hipError_t launch_keep(const CacheView& c, const StepView& st, const uint32_t* kept, const uint32_t* kept_count,
                        uint32_t max_kept, hipStream_t s);

@@ -1581,7 +1581,7 @@ mx4_status mx4_cache_copy_pages(mx4_context* ctx, const mx4_kv_cache* cache, con
     if (!aligned(pairs, 4)) return fail(MX4_ERR_ARGUMENT, "pairs must be 4-byte aligned");
     if (count == 0) return MX4_OK;
     DeviceGuard g(ctx->device);
-    const hipError_t e = mx4::launch_copy_pages(c, pairs, count, ctx->cus, ctx->stream);
+    const hipError_t e = mx4::launch_copy_pages(c, pairs, count, ctx->stream);
     if (e != hipSuccess) return fail(MX4_ERR_DEVICE, "page copy launch failed: %s", hipGetErrorString(e));
     return MX4_OK;
 }
