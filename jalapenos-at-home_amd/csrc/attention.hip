@@ -224,112 +224,105 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attention_rows_kernel(A
             for (uint32_t x = 0; x < D / 16; ++x) add_to_stored(a, c, n, key, kv, row, row, d0 + x, part);
 }
 
-// Partial rows of the chunks from .. to - 1 against their largest maximum, by one wave: what
-// the lanes with part_of == 0 then hold in o (channels d .. d + 3) and all in top and l. A row is
-// D / 4 lanes of four channels, so a wave has 256 / D chunks side by side and eight such sets
-// in flight; the order of the sums is fixed. stats, part: the row's in the first chunk's slot.
-template <int D>
-__device__ __forceinline__ void join_chunks(const float* stats, const float* part, uint64_t stride, uint32_t from, uint32_t to,
-                                            float& top, float& l, f32x4& o) {
-    constexpr uint32_t SIDE = 256 / D, DEEP = 8;
-    const uint32_t lane = threadIdx.x & 63, part_of = lane / (D / 4);
+// Four channels of a row: the partial rows of its chunks first, first + step, .. under one
+// maximum, DEEP in flight. stats, part: the row's in the first chunk's slot.
+template <int DEEP>
+__device__ __forceinline__ void join_chunks(const float* stats, const float* part, uint32_t stride, uint32_t first, uint32_t step,
+                                            uint32_t chunks, float& top, float& l, f32x4& o) {
     top = kNoMax;
     l = 0.0f;
     o = f32x4{0, 0, 0, 0};
-    for (uint32_t i = from + lane; i < to; i += 64) top = fmaxf(top, stats[i * stride]);
-    for (uint32_t w0 = from; w0 < to; w0 += 64) {
-        const uint32_t left = min(to - w0, 64u);
-        const float* mine = stats + (w0 + min(lane, left - 1)) * stride;
-        const float mine_top = mine[0], mine_l = mine[1];
-        float weight = 0.0f;
-        for (uint32_t i0 = 0; i0 < left; i0 += SIDE * DEEP) {
-            f32x4 x[DEEP];
+    for (uint32_t i = first; i < chunks; i += DEEP * step) {
+        float2 st[DEEP];
+        f32x4 x[DEEP];
 #pragma unroll
-            for (uint32_t u = 0; u < DEEP; ++u)
-                if (i0 + u * SIDE < left)
-                    x[u] = *reinterpret_cast<const f32x4_near*>(part + (w0 + min(i0 + u * SIDE + part_of, left - 1)) * stride);
-            if (i0 == 0) {
-                if (w0 == from)
-#pragma unroll
-                    for (int off = 1; off < 64; off *= 2) top = fmaxf(top, __shfl_xor(top, off));
-                weight = lane < left ? __builtin_amdgcn_exp2f(mine_top - top) : 0.0f;
-                l += lane < left ? weight * mine_l : 0.0f;
-            }
-#pragma unroll
-            for (uint32_t u = 0; u < DEEP; ++u)
-                if (i0 + u * SIDE < left) {
-                    const uint32_t at = i0 + u * SIDE + part_of;
-                    const float by = __shfl(weight, at & 63);
-                    if (at < left)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(by, x[u][e], o[e]);
-                }
+        for (int u = 0; u < DEEP; ++u) {
+            const uint64_t at = (uint64_t)min(i + u * step, chunks - 1) * stride;
+            st[u] = *reinterpret_cast<const float2*>(stats + at);
+            x[u] = *reinterpret_cast<const f32x4_near*>(part + at);
         }
+        float now = top;
+#pragma unroll
+        for (int u = 0; u < DEEP; ++u) now = fmaxf(now, st[u].x);
+        const float keep = __builtin_amdgcn_exp2f(top - now);
+        l *= keep;
+        o *= keep;
+        top = now;
+#pragma unroll
+        for (int u = 0; u < DEEP; ++u)
+            if (i + u * step < chunks) {
+                const float by = __builtin_amdgcn_exp2f(st[u].x - now);
+                l = __builtin_fmaf(by, st[u].y, l);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(by, x[u][e], o[e]);
+            }
     }
-#pragma unroll
-    for (uint32_t off = D / 4; off < 64; off *= 2)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], off);
-#pragma unroll
-    for (int off = 1; off < 64; off *= 2) l += __shfl_xor(l, off);
 }
 
-// A wave takes a row of a cut row block, the next one 4 gridDim.z further; a row of more than
-// kWaveChunks chunks (a wave's loads in one go) is the whole workgroup's, its waves' parts
-// joined once more in LDS: one user's 33 chunks in 4.2 us, by a wave in 5.2. (A launch of its
-// own: joining in the last workgroup to arrive takes a release and an acquire past the
-// XCD's L2 from every one, 14 us more for one user's decode and 170 for 32 users'.) Bound: the
-// partial rows' bytes where they are many -- 61 chunks of 100 rows and 8 kv heads, 26 MB, 8 us.
-constexpr uint32_t kWaveChunks = 16;
+// The chunks' partial rows of cut row blocks against their largest maximum, in a fixed order. D / 4
+// threads take a row (four channels each, which need nothing of one another), so a workgroup
+// 1024 / D of them, and the next ones as many times gridDim.z further; a row of more than
+// kRowChunks chunks is the whole workgroup's, its parts joined once more in LDS. (A launch of its
+// own: joining in the last workgroup to arrive takes a release and an acquire past the XCD's L2
+// from every one, 14 us more for one user's decode and 170 for 32 users'.)
+constexpr uint32_t kRowChunks = 16;
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a, Split split, uint32_t slot_rows) {
-    __shared__ float parts[4][D], tops[4], sums[4];
-    const uint32_t lane = threadIdx.x & 63, d = lane % (D / 4) * 4;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr uint32_t ROWS = 1024 / D;
+    __shared__ __align__(16) float parts[ROWS][D];
+    __shared__ float tops[ROWS], sums[ROWS];
+    const uint32_t mine = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
     const uint32_t kvs = a.cache.kv_heads, kv = blockIdx.y, group = a.q_heads / kvs;
     Chunk c;
     Lengths n;
     if (!find_chunk(a.step, table_room(a.step, a.cache.page_shift), group, split, blockIdx.x, true, c, n)) return;
     const uint32_t row0 = c.block * split.rows, rows = min(split.rows, n.fresh * group - row0);
-    const uint64_t stride = (uint64_t)kvs * slot_rows * (D + 2);
-    const float* slot = a.part + ((uint64_t)c.slot * kvs + kv) * slot_rows * (D + 2);
-    const bool alone = c.chunks <= kWaveChunks;
-    const uint32_t share = alone ? c.chunks : (c.chunks + 3) / 4, from = alone ? 0 : min(wave * share, c.chunks);
-    const uint32_t by_four = alone ? 4 : 1;
-    for (uint32_t row = blockIdx.z * by_four + (alone ? wave : 0); row < rows; row += gridDim.z * by_four) {
-        float top, l;
-        f32x4 o;
-        join_chunks<D>(slot + slot_rows * D + 2 * row, slot + row * D + d, stride, from, min(from + share, c.chunks), top, l, o);
-        if (!alone) {
-            if (lane < D / 4) *reinterpret_cast<f32x4*>(&parts[wave][d]) = o;
-            if (lane == 0) {
-                tops[wave] = top;
-                sums[wave] = l;
-            }
-            __syncthreads();
-            if (wave == 0) {
-                const float now = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-                l = 0.0f;
-                o = f32x4{0, 0, 0, 0};
+    const uint32_t stride = kvs * slot_rows * (D + 2);  // (within the scratch)
+    const float* slot = a.part + (uint64_t)(c.slot * kvs + kv) * slot_rows * (D + 2);
+    float top, l;
+    f32x4 o;
+    auto store = [&](uint32_t row) {
+        const float by = l == 0.0f ? 0.0f : 1.0f / l;
+        const uint32_t r = row0 + row;
+        __bf16 b[4];
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float by = __builtin_amdgcn_exp2f(tops[w] - now);
-                    l = __builtin_fmaf(by, sums[w], l);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(by, parts[w][d + e], o[e]);
-                }
-            }
-            __syncthreads();
+        for (int e = 0; e < 4; ++e) b[e] = (__bf16)(o[e] * by);
+        *reinterpret_cast<uint2*>(a.out + (uint64_t)(n.first + r / group) * a.out_stride + (uint64_t)(kv * group + r % group) * D + d) =
+            __builtin_bit_cast(uint2, b);
+    };
+    if (c.chunks <= kRowChunks) {
+        for (uint32_t row = blockIdx.z * ROWS + mine; row < rows; row += gridDim.z * ROWS) {
+            const float *stats = slot + slot_rows * D + 2 * row, *part = slot + row * D + d;
+            if (c.chunks <= 4) join_chunks<4>(stats, part, stride, 0, 1, c.chunks, top, l, o);
+            else join_chunks<8>(stats, part, stride, 0, 1, c.chunks, top, l, o);
+            store(row);
         }
-        if (lane < D / 4 && (alone || wave == 0)) {
-            const float by = l == 0.0f ? 0.0f : 1.0f / l;
-            const uint32_t r = row0 + row;
-            __bf16 b[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) b[e] = (__bf16)(o[e] * by);
-            *reinterpret_cast<uint2*>(a.out + (uint64_t)(n.first + r / group) * a.out_stride + (uint64_t)(kv * group + r % group) * D + d) =
-                __builtin_bit_cast(uint2, b);
+        return;
+    }
+    for (uint32_t row = blockIdx.z; row < rows; row += gridDim.z) {
+        join_chunks<8>(slot + slot_rows * D + 2 * row, slot + row * D + d, stride, mine, ROWS, c.chunks, top, l, o);
+        *reinterpret_cast<f32x4*>(&parts[mine][d]) = o;
+        if (d == 0) {
+            tops[mine] = top;
+            sums[mine] = l;
         }
+        __syncthreads();
+        if (mine == 0) {
+            top = kNoMax;
+#pragma unroll
+            for (uint32_t i = 0; i < ROWS; ++i) top = fmaxf(top, tops[i]);
+            l = 0.0f;
+            o = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t i = 0; i < ROWS; ++i) {
+                const float by = __builtin_amdgcn_exp2f(tops[i] - top);
+                l = __builtin_fmaf(by, sums[i], l);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(by, parts[i][d + e], o[e]);
+            }
+            store(row);
+        }
+        __syncthreads();
     }
 }
 
@@ -356,9 +349,10 @@ hipError_t launch_join(const AttentionArgs& a, const Split& split, uint64_t bloc
     // (a table of one unit's pages holds no sequence that could be cut)
     if (split.target > 1 && (uint64_t)a.step.table_stride << a.cache.page_shift > kUnit) {
         const uint32_t cut = (uint32_t)(blocks < split.target ? blocks : split.target), kv = a.cache.kv_heads;
-        // a row a wave, or a workgroup where a row may have many chunks; each workgroup has to find its
-        // row block first, so not more than kJoins
-        const uint32_t most = kJoins / (cut * kv), whole = split.target > kWaveChunks * cut ? slot_rows : (slot_rows + 3) / 4, z = most < 1 ? 1 : most > whole ? whole : most;
+        // each workgroup has to find its row block first, so not more than kJoins
+        const uint32_t at_once = split.target > kRowChunks * cut ? 1 : 1024 / a.cache.head_dim;  // rows (fewer than may be)
+        const uint32_t most = kJoins / (cut * kv), whole = (slot_rows + at_once - 1) / at_once;
+        const uint32_t z = most < 1 ? 1 : most > whole ? whole : most;
         const dim3 grid(cut, kv, z);
         if (a.cache.head_dim == 64) join_kernel<64><<<grid, dim3(256), 0, a.stream>>>(a, split, slot_rows);
         if (a.cache.head_dim == 128) join_kernel<128><<<grid, dim3(256), 0, a.stream>>>(a, split, slot_rows);
