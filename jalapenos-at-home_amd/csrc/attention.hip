@@ -276,6 +276,8 @@ __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a, Split split,
     Chunk c;
     Lengths n;
     if (!find_chunk(a.step, table_room(a.step, a.cache.page_shift), group, split, blockIdx.x, true, c, n)) return;
+    c.chunks = chunks_of_block(c, keys_of_block(a, n, group, split.rows, c.block));
+    if (c.chunks == 1) return;
     const uint32_t row0 = c.block * split.rows, rows = min(split.rows, n.fresh * group - row0);
     const uint32_t stride = kvs * slot_rows * (D + 2);  // (within the scratch)
     const float* slot = a.part + (uint64_t)(c.slot * kvs + kv) * slot_rows * (D + 2);

@@ -110,6 +110,17 @@ __device__ __forceinline__ bool find_chunk(const StepView& st, uint32_t room, ui
     return false;
 }
 
+// Keys up to the last that a row block sees (of a chain: its last row), and the chunks that hold
+// them: the block's later ones have nothing to do, and with one the block is not cut.
+__device__ __forceinline__ uint32_t keys_of_block(const AttentionArgs& a, const Lengths& n, uint32_t group, uint32_t rows,
+                                                  uint32_t block) {
+    const uint32_t last_row = min((block + 1) * rows, n.fresh * group) - 1;
+    return a.tree ? n.keys : min(n.keys, n.before + last_row / group + 1);
+}
+__device__ __forceinline__ uint32_t chunks_of_block(const Chunk& c, uint32_t keys) {
+    return max(((keys + kUnit - 1) / kUnit + c.cu - 1) / c.cu, 1u);
+}
+
 // The keys that row (first + i) sees of the 32 from k0 on, one bit each.
 __device__ __forceinline__ uint32_t seen_window(const AttentionArgs& a, const Lengths& n, uint32_t i, uint32_t k0) {
     const int64_t j0 = (int64_t)k0 - n.before;  // place among the new tokens

@@ -189,10 +189,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
     Lengths n;
     if (!find_chunk(a.step, room, group, split, blockIdx.x / kvs, false, c, n)) return;
     const uint32_t row0 = c.block * ROWS, all_rows = n.fresh * group;
-    // chains: the keys that the block's last row sees; and how far all rows of the block see
-    const uint32_t last_row = min(row0 + ROWS, all_rows) - 1;
-    const uint32_t end_key = a.tree ? n.keys : min(n.keys, n.before + last_row / group + 1);
-    const uint32_t clear = a.tree ? n.before : min(n.keys, n.before + row0 / group + 1);
+    const uint32_t end_key = keys_of_block(a, n, group, ROWS, c.block);
+    c.chunks = chunks_of_block(c, end_key);
+    if (c.chunk >= c.chunks) return;
+    const uint32_t clear = a.tree ? n.before : min(n.keys, n.before + row0 / group + 1);  // all rows of the block see these
     const uint32_t tile0 = c.chunk * c.cu * (kUnit / kTile);
     const uint32_t tile_end = min(tile0 + c.cu * (kUnit / kTile), (end_key + kTile - 1) / kTile);
     Stage<D> st;
