@@ -447,8 +447,8 @@ typedef struct mx4_kv_cache {
  * pass reads their values of each replay; max_tokens is the most tokens of the
  * call that any sequence has (or a bound of it). Nothing is accessed outside
  * the cache whatever the arrays hold: a page number past the cache is never
- * written (reading, it stands for the last page), positions past the table are
- * left out, and so are a sequence's tokens past max_tokens (their outputs are
+ * written (reading, it stands for the last page), positions past the table (or
+ * past 2^28 - 1 for attention) are left out, and so are a sequence's tokens past max_tokens (their outputs are
  * not written). */
 typedef struct mx4_batch {
     uint32_t seqs, tokens, max_tokens, table_stride;

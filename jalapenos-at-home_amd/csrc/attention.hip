@@ -47,6 +47,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attention_rows_kernel(A
     const uint32_t room = table_room(a.step, shift);
     Chunk c;
     Lengths n;
+    split.fit = false;
     if (!find_chunk(a.step, room, group, split, blockIdx.x, false, c, n)) return;
     const uint32_t rows = n.fresh * group;
     const uint32_t step0 = c.chunk * c.cu * (kUnit / 32), step_end = min(step0 + c.cu * (kUnit / 32), (n.keys + 31) / 32);
@@ -336,7 +337,7 @@ hipError_t launch_rows(const AttentionArgs& a, int cus) {
     // 40000 keys (32 / 8 heads of 128) take 42.7 / 45.2 us, 16 users of 100 .. 8000 keys 48 / 53,
     // 32 of them 66 / 63, 64 of them 105 / 101; with two 44.7, 49, 64 and 113.
     const uint64_t each = (uint64_t)a.step.seqs * kv < (uint64_t)cus ? 3 : 4;
-    const Split split{split_target(a, each * cus / kv, a.step.seqs, slot_rows), 16};
+    const Split split{split_target(a, each * cus / kv, a.step.seqs, slot_rows), 16, false};
     attention_rows_kernel<D><<<dim3(most_chunks(a, split.target, a.step.seqs), kv), dim3(256), 0, a.stream>>>(a, split, slot_rows);
     return launch_join(a, split, a.step.seqs, slot_rows);
 }

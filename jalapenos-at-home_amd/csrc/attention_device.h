@@ -14,15 +14,17 @@ constexpr uint32_t kUnit = 128;  // keys: the grain in which a sequence is cut a
 
 // ------------------------------------------------------------- the split along the keys
 
-constexpr uint32_t kUncut = 1u << 24;  // units: 2^31 keys, more than a sequence has
+constexpr uint32_t kUncut = 1u << 21;  // units: 2^28 keys, the most that a sequence has
 
-// How the step's work is cut. Every (row block, kv head) of a sequence has
-// ceil(units / cu) chunks of cu units; cu makes about `target` chunks a kv head of
-// the whole step, from the lengths in device memory; a target of 1 cuts nothing. Chunks of cut rows leave
-// partial results in slots, joined by join_kernel. A sequence's last row block
-// comes first: in a prompt it has the most keys.
+// How the step's work is cut. Every (row block, kv head) of a sequence has as many chunks of cu
+// units as it has keys for, evened out among them; cu makes about `target` chunks a kv head of the
+// whole step, from the lengths in device memory; a target of 1 cuts nothing. With `fit` a step makes
+// no more than that where it can, and a sequence whose way a cut would shorten by one unit is left
+// whole. Chunks of cut rows leave partial results in slots, joined by join_kernel. A
+// sequence's last row block comes first: in a prompt it has the most keys.
 struct Split {
     uint32_t target, rows;  // rows: of a row block
+    bool fit;
 };
 struct Chunk {
     uint32_t s, block, chunk, chunks, slot, cu;  // slot: of the row block's first chunk, a kv head's numbering
@@ -65,6 +67,13 @@ __device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {
 
 __device__ __forceinline__ uint32_t lane_of(uint32_t v, uint32_t lane) { return __builtin_amdgcn_readlane(v, lane); }
 
+// a / b, rounded up, of 1 <= a <= 2^21 units: the quotient of a - 1/2 keeps off the whole numbers by
+// 1/2 b, more than its error. (Where a kernel begins, every instruction is waited for: those of
+// the whole-number divisions took 0.5 us of a small call.)
+__device__ __forceinline__ uint32_t div_up(uint32_t a, uint32_t b) {
+    return (uint32_t)(((float)a - 0.5f) * __builtin_amdgcn_rcpf((float)b)) + 1;
+}
+
 // The chunk that is number `item` of its kv head or, with `cut`, the first chunk of the
 // kv head's cut row block number `item`, and its sequence's lengths. False: there is
 // none. Called by whole waves; everything it gives is the same in all lanes.
@@ -72,7 +81,7 @@ __device__ __forceinline__ bool find_chunk(const StepView& st, uint32_t room, ui
                                            bool cut, Chunk& c, Lengths& n) {
     const uint32_t lane = threadIdx.x & 63;
     Lengths mine{};
-    uint32_t units = 0, blocks = 0, total = 0;
+    uint32_t units = 0, blocks = 0, chunks = 0, total = 0, all_blocks = 0, cu = kUncut;
     auto shape = [&](uint32_t s) {
         units = blocks = 0;
         if (s >= st.seqs) return;
@@ -81,15 +90,38 @@ __device__ __forceinline__ bool find_chunk(const StepView& st, uint32_t room, ui
         units = max((mine.keys + kUnit - 1) / kUnit, 1u);
         blocks = (mine.fresh * group + split.rows - 1) / split.rows;
     };
-    for (uint32_t s0 = 0; s0 < st.seqs; s0 += 64) {
-        shape(s0 + lane);
-        if (split.target > 1) total += lane_of(wave_prefix(units * blocks), 63);
+    auto cut_up = [&] { chunks = units > cu + split.fit ? div_up(units, cu) : min(units, 1u); };
+    if (split.target > 1) {
+        for (uint32_t s0 = 0; s0 < st.seqs; s0 += 64) {
+            shape(s0 + lane);
+            total += lane_of(wave_prefix(units * blocks), 63);
+            if (split.fit) all_blocks += lane_of(wave_prefix(blocks), 63);
+        }
+        cu = max((total + split.target - 1) / split.target, 1u);
+        // More row blocks than that make several rounds, where short ones fill what long ones leave.
+        if (all_blocks >= split.target) cu *= 2;
+        cut_up();
+        for (int i = 0; i < 4 && split.fit && all_blocks < split.target; ++i) {
+            uint32_t count = 0;
+            for (uint32_t s0 = 0; s0 < st.seqs; s0 += 64) {
+                if (st.seqs > 64) {
+                    shape(s0 + lane);
+                    cut_up();
+                }
+                count += lane_of(wave_prefix(chunks * blocks), 63);
+            }
+            if (count <= split.target) break;
+            cu = (uint32_t)((float)cu * (float)count * __builtin_amdgcn_rcpf((float)split.target)) + 1;
+            cut_up();
+        }
     }
-    c.cu = split.target > 1 ? max((total + split.target - 1) / split.target, 1u) : kUncut;
     uint32_t items = 0, slots = 0;
     for (uint32_t s0 = 0; s0 < st.seqs; s0 += 64) {
-        if (st.seqs > 64) shape(s0 + lane);
-        const uint32_t chunks = (units + c.cu - 1) / c.cu, in_slots = chunks > 1 ? chunks * blocks : 0;
+        if (st.seqs > 64 || split.target <= 1) {
+            shape(s0 + lane);
+            cut_up();
+        }
+        const uint32_t in_slots = chunks > 1 ? chunks * blocks : 0;
         const uint32_t count = cut ? (chunks > 1 ? blocks : 0) : chunks * blocks;
         const uint32_t upto = items + wave_prefix(count), slots_upto = slots + wave_prefix(in_slots);
         const uint64_t hit = __ballot(item < upto);
@@ -97,6 +129,7 @@ __device__ __forceinline__ bool find_chunk(const StepView& st, uint32_t room, ui
             const uint32_t at = __ffsll((unsigned long long)hit) - 1;
             c.s = s0 + at;
             c.chunks = lane_of(chunks, at);
+            c.cu = c.chunks > 1 ? div_up(lane_of(units, at), c.chunks) : kUncut;
             const uint32_t in = item - (lane_of(upto, at) - lane_of(count, at)), block = cut ? in : in / c.chunks;
             c.block = lane_of(blocks, at) - 1 - block;
             c.chunk = cut ? 0 : in - block * c.chunks;
@@ -118,7 +151,7 @@ __device__ __forceinline__ uint32_t keys_of_block(const AttentionArgs& a, const 
     return a.tree ? n.keys : min(n.keys, n.before + last_row / group + 1);
 }
 __device__ __forceinline__ uint32_t chunks_of_block(const Chunk& c, uint32_t keys) {
-    return max(((keys + kUnit - 1) / kUnit + c.cu - 1) / c.cu, 1u);
+    return c.chunks > 1 && keys != 0 ? div_up((keys + kUnit - 1) / kUnit, c.cu) : 1;
 }
 
 // The keys that row (first + i) sees of the 32 from k0 on, one bit each.

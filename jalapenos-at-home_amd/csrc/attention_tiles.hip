@@ -187,6 +187,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
     const uint32_t room = table_room(a.step, shift);
     Chunk c;
     Lengths n;
+    split.fit = true;
     if (!find_chunk(a.step, room, group, split, blockIdx.x / kvs, false, c, n)) return;
     const uint32_t row0 = c.block * ROWS, all_rows = n.fresh * group;
     const uint32_t end_key = keys_of_block(a, n, group, ROWS, c.block);
@@ -395,12 +396,13 @@ hipError_t launch_tiles(const AttentionArgs& a, int cus) {
     // row blocks of a kv head: the tokens' whole ones, and a partial one a sequence
     const uint64_t whole = (uint64_t)a.step.tokens * group / ROWS, blocks = whole + a.step.seqs;
     const uint32_t slot_rows = rows < ROWS ? (uint32_t)rows : ROWS;
-    // Two workgroups a CU, as many as are there at a time: 12 trees of 9 .. 32 tokens take 35 us,
-    // with one a CU 41; 25 tokens behind 39000 take 49 and 47 (half the partial rows), with three
-    // 61. One sequence of as many row blocks would not be cut, which saves the join's launch.
+    // Two workgroups a CU, as many as are there at a time: 12 trees of 9 .. 32 tokens take 33 us,
+    // with one or three a CU 38 and 44; 7 trees of 48 tokens behind 13600 keys (64 / 8 heads) 186,
+    // 287 and 207; 25 tokens behind 39000 46, 44 (half the partial rows) and 56. One sequence whose
+    // row blocks would not fit twice is left whole, which saves the join's launch.
     uint32_t target = split_target(a, 2ull * cus / kv, blocks, slot_rows);
-    if (a.step.seqs == 1 && whole >= target) target = 1;
-    const Split split{target, ROWS};
+    if (a.step.seqs == 1 && 2 * (whole + 1) > target) target = 1;
+    const Split split{target, ROWS, true};
     attention_tiles_kernel<D><<<dim3(most_chunks(a, split.target, blocks) * kv), dim3(256), 0, a.stream>>>(a, split, slot_rows);
     return launch_join(a, split, blocks, slot_rows);
 }

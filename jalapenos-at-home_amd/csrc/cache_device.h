@@ -31,10 +31,10 @@ __device__ __forceinline__ void tokens_of(const StepView& st, uint32_t s, uint32
     count = b > a ? min(b - a, st.max_tokens) : 0;
 }
 
-// Positions that a sequence's row of the page table can hold, at most 2^31.
+// Positions that a sequence's row of the page table can hold, at most 2^28.
 __device__ __forceinline__ uint32_t table_room(const StepView& st, uint32_t page_shift) {
     const uint64_t room = (uint64_t)st.table_stride << page_shift;
-    return room < 0x80000000ull ? (uint32_t)room : 0x80000000u;
+    return room < 0x10000000ull ? (uint32_t)room : 0x10000000u;
 }
 
 }  // namespace mx4

@@ -158,6 +158,9 @@ constexpr uint32_t kArgmaxPartials = 8192;
 // f32 output); the skinny kernel's split takes at most 4096 tiles of 1 KiB
 // of it (four K slices of up to 8192 rows at 32 tokens).
 constexpr uint64_t kSplitPartBytes = 32ull << 20;
+// What attention may use of it: the partial rows of two workgroups a CU and of as many row blocks
+// again, 128 rows of 256 floats each.
+constexpr uint64_t kAttentionPartBytes = 136ull << 20;
 constexpr uint32_t kSplitPartTiles = 4096;
 constexpr uint32_t kSplitCounts = 4096;
 
@@ -527,7 +530,7 @@ mx4_status mx4_create(int device, mx4_context** out) {
         hipEventCreate(&ctx->ev0) != hipSuccess || hipEventCreate(&ctx->ev1) != hipSuccess ||
         hipMalloc((void**)&ctx->flags, (kMinMaxAt + 2 * mx4::kMinMaxBlocks) * 4) != hipSuccess ||
         hipMalloc((void**)&ctx->am_partial, kArgmaxPartials * sizeof(uint64_t)) != hipSuccess ||
-        hipMalloc((void**)&ctx->split_part, (size_t)kSplitPartBytes) != hipSuccess ||
+        hipMalloc((void**)&ctx->split_part, (size_t)kAttentionPartBytes) != hipSuccess ||
         hipMalloc((void**)&ctx->split_count, kSplitCounts * sizeof(uint32_t)) != hipSuccess ||
         hipMemsetAsync(ctx->split_count, 0, kSplitCounts * sizeof(uint32_t), ctx->own) != hipSuccess ||
         hipStreamSynchronize(ctx->own) != hipSuccess) {
@@ -1565,7 +1568,7 @@ mx4_status mx4_attention(mx4_context* ctx, const uint16_t* q, uint64_t q_stride,
     a.tree_words = tree_words;
     a.scale = scale > 0.0f ? scale : 1.0f / std::sqrt((float)cache->head_dim);
     a.part = ctx->split_part;
-    a.part_bytes = kSplitPartBytes;
+    a.part_bytes = kAttentionPartBytes;
     a.stream = ctx->stream;
     DeviceGuard g(ctx->device);
     const hipError_t e = mx4::launch_attention(a, ctx->cus);

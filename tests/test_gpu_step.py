@@ -253,6 +253,8 @@ def test_attention_masked_places_have_no_part(mx4, ctx, new, cached, bad):
     ([1], [20000], 8, 1, 128, 16), ([40], [9000], 4, 1, 64, 16),
     # one sequence of more row blocks than the device takes at a time, and beside a longer one
     ([600], [0], 128, 128, 64, 16), ([600, 1], [0, 3000], 64, 64, 64, 16),
+    # chunks that have to grow to fit, of more than a wave's lanes; more row blocks than fit, and a long way
+    ([40] * 100, [560] * 100, 4, 1, 64, 16), ([600, 1, 500], [0, 3000, 20], 64, 64, 64, 16),
 ])
 def test_attention_batches(mx4, ctx, new, cached, hq, hk, d, page):
     rng = np.random.default_rng(hq * 1000 + d + sum(new) + sum(cached))
