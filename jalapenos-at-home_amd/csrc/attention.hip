@@ -32,7 +32,7 @@ typedef float f32x4_near __attribute__((ext_vector_type(4), aligned(8)));  // (a
 //
 // Bound: the cache's bytes. 32 users of 100 .. 8000 keys (32 / 8 heads of 128, 257 MB): 58 us,
 // 4.4 TB/s, where a large copy makes 4.9. One user's 4111 keys (16 / 8 heads, 17 MB) are latency:
-// 9 us, of which the launch is 3, the rest the lengths, the page table and the keys one after
+// 8 us, of which the launch is 3, the rest the lengths, the page table and the keys one after
 // the other and the four waves' rows through LDS.
 template <int D>
 __global__ __launch_bounds__(256, D <= 128 ? 3 : 1) void attention_rows_kernel(AttentionArgs a, Split split, uint32_t slot_rows) {
@@ -263,10 +263,13 @@ __device__ __forceinline__ void join_chunks(const float* stats, const float* par
 // The chunks' partial rows of cut row blocks against their largest maximum, in a fixed order. D / 4
 // threads take a row (four channels each, which need nothing of one another), so a workgroup
 // 1024 / D of them, and the next ones as many times gridDim.z further; a row of more than
-// kRowChunks chunks is the whole workgroup's, its parts joined once more in LDS. (A launch of its
-// own: joining in the last workgroup to arrive takes a release and an acquire past the XCD's L2
-// from every one, 14 us more for one user's decode and 170 for 32 users'.)
-constexpr uint32_t kRowChunks = 16;
+// kRowChunks chunks is the whole workgroup's, its parts joined once more in LDS (32 users' decode and
+// 12 trees of 9 .. 32 tokens take 63.0 and 32.4 us with 16 or 32, 66.0 and 35.4 with 8; 5 trees of
+// 22 chunks a row 50.2 with 16, 48.7 with 32). Bound: 61 chunks of 100 rows and 8 kv heads (26 MB)
+// 7 us, their bytes; one user's 33 chunks 4 us, the launch and two dependent loads. (A launch of
+// its own: joining in the last workgroup to arrive takes a release and an acquire past the
+// XCD's L2 from every one, 14 us more for one user's decode and 170 for 32 users'.)
+constexpr uint32_t kRowChunks = 32;
 template <int D>
 __global__ __launch_bounds__(256) void join_kernel(AttentionArgs a, Split split, uint32_t slot_rows) {
     constexpr uint32_t ROWS = 1024 / D;
@@ -342,9 +345,9 @@ hipError_t launch_rows(const AttentionArgs& a, int cus) {
     return launch_join(a, split, a.step.seqs, slot_rows);
 }
 
-// Workgroups of a join, past a row block's first each: 12 trees of 9 .. 32 tokens take 34.9 us,
-// with half as many 35.6, with twice as many 36.4.
-constexpr uint32_t kJoins = 2048;
+// Workgroups of a join: 12 trees of 9 .. 32 tokens take 31.4 us, chunks of prompts 41.5, 5 trees of 22
+// chunks a row 50.2; with twice as many 32.4, 42.5 and 48.9, with four times 32.4, 44.1 and 50.5.
+constexpr uint32_t kJoins = 1024;
 
 }  // namespace
 

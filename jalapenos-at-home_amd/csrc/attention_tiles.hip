@@ -162,11 +162,11 @@ struct Stage {
 // The maximum is not looked for: a row whose weights' sum passes 2^kSlack has to raise it,
 // and takes its weights again.
 //
-// Bound: a prompt's 8001 tokens (32 / 8 heads of 128, 524 GFLOP behind the mask) take 515 us, 1018
+// Bound: a prompt's 8001 tokens (32 / 8 heads of 128, 524 GFLOP behind the mask) take 512 us, 1024
 // TFLOP/s; a large library product makes 1239, and as there the clock falls under the load (to
 // 1.6 GHz with the matrix cores half busy). Two workgroups share a CU, which fills what the one
 // leaves; with one the prompt takes 800 us, with 64 rows a wave (one wave a SIMD) 571. Trees of 9
-// .. 32 tokens (91 MB of cache) are bound by its bytes, 27 us of 35 with the join; chunks of
+// .. 32 tokens (94 MB of cache) are bound by its bytes, 26 us of 31 with the join; chunks of
 // prompts (1 .. 900 tokens) by the last row block's way through its keys, 1.1 us a tile.
 //
 // A weight of zero times an infinite or NaN value would spread NaN to rows that do not
@@ -396,7 +396,7 @@ hipError_t launch_tiles(const AttentionArgs& a, int cus) {
     // row blocks of a kv head: the tokens' whole ones, and a partial one a sequence
     const uint64_t whole = (uint64_t)a.step.tokens * group / ROWS, blocks = whole + a.step.seqs;
     const uint32_t slot_rows = rows < ROWS ? (uint32_t)rows : ROWS;
-    // Two workgroups a CU, as many as are there at a time: 12 trees of 9 .. 32 tokens take 33 us,
+    // Two workgroups a CU, as many as are there at a time: 12 trees of 9 .. 32 tokens take 32 us,
     // with one or three a CU 38 and 44; 7 trees of 48 tokens behind 13600 keys (64 / 8 heads) 186,
     // 287 and 207; 25 tokens behind 39000 46, 44 (half the partial rows) and 56. One sequence whose
     // row blocks would not fit twice is left whole, which saves the join's launch.
