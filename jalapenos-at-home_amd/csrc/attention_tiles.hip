@@ -164,7 +164,7 @@ struct Stage {
 //
 // Bound: a prompt's 8001 tokens (32 / 8 heads of 128, 524 GFLOP behind the mask) take 512 us, 1024
 // TFLOP/s; a large library product makes 1239, and as there the clock falls under the load (to
-// 1.6 GHz with the matrix cores half busy). Two workgroups share a CU, which fills what the one
+// 1.7 GHz with the matrix cores half busy). Two workgroups share a CU, which fills what the one
 // leaves; with one the prompt takes 800 us, with 64 rows a wave (one wave a SIMD) 571. Trees of 9
 // .. 32 tokens (94 MB of cache) are bound by its bytes, 26 us of 31 with the join; chunks of
 // prompts (1 .. 900 tokens) by the last row block's way through its keys, 1.1 us a tile.
