@@ -103,7 +103,8 @@ void qwen_hip_set_cache_limit(void *context, uint64_t bytes);
 
 /* gpu_create (engine/src/gpu.m:27-49): binds HIP device `device` and creates
  * the context's stream (default priority) and its device scratch (argmax
- * partials, and 32 MiB of split-K partial tiles with their arrival counts).
+ * partials, and 136 MiB for the partial tiles and rows of split work -- matrix
+ * products use 32 MiB of it -- with their arrival counts).
  * The scratch is shared by every call on the context, so calls on one context
  * must stay ordered: after mx4_set_stream, work still queued on the previous
  * stream must finish before the new stream runs more. */
