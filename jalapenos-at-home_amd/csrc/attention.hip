@@ -340,7 +340,7 @@ hipError_t launch_rows(const AttentionArgs& a, int cus) {
     // 40000 keys (32 / 8 heads of 128) take 42.7 / 45.2 us, 16 users of 100 .. 8000 keys 48 / 53,
     // 32 of them 66 / 63, 64 of them 105 / 101; with two 44.7, 49, 64 and 113.
     const uint64_t each = (uint64_t)a.step.seqs * kv < (uint64_t)cus ? 3 : 4;
-    const Split split{split_target(a, each * cus / kv, a.step.seqs, slot_rows), 16, false};
+    const Split split{split_target(a, each * cus / kv, a.step.seqs, slot_rows), 16, (uint32_t)split_slots(a, slot_rows), false};
     attention_rows_kernel<D><<<dim3(most_chunks(a, split.target, a.step.seqs), kv), dim3(256), 0, a.stream>>>(a, split, slot_rows);
     return launch_join(a, split, a.step.seqs, slot_rows);
 }

@@ -23,7 +23,7 @@ constexpr uint32_t kUncut = 1u << 21;  // units: 2^28 keys, the most that a sequ
 // whole. Chunks of cut rows leave partial results in slots, joined by join_kernel. A
 // sequence's last row block comes first: in a prompt it has the most keys.
 struct Split {
-    uint32_t target, rows;  // rows: of a row block
+    uint32_t target, rows, slots;  // rows: of a row block; slots: that the scratch has, a kv head
     bool fit;
 };
 struct Chunk {
@@ -134,6 +134,9 @@ __device__ __forceinline__ bool find_chunk(const StepView& st, uint32_t room, ui
             c.block = lane_of(blocks, at) - 1 - block;
             c.chunk = cut ? 0 : in - block * c.chunks;
             c.slot = lane_of(slots_upto, at) - lane_of(in_slots, at) + block * c.chunks;
+            // (starts that are not ascending may make more of everything than there is room or count for)
+            if (block >= lane_of(blocks, at)) return false;
+            if (c.chunks > 1 && (c.chunks > split.slots || c.slot > split.slots - c.chunks)) return false;
             n = {lane_of(mine.first, at), lane_of(mine.fresh, at), lane_of(mine.before, at), lane_of(mine.keys, at)};
             return true;
         }
@@ -198,10 +201,12 @@ inline uint64_t most_units(const AttentionArgs& a) {  // that a sequence of this
     const uint64_t room = (uint64_t)a.step.table_stride << a.cache.page_shift;
     return room < kUnit ? 1 : (room + kUnit - 1) / kUnit;
 }
+inline uint64_t split_slots(const AttentionArgs& a, uint32_t slot_rows) {
+    return a.part_bytes / ((uint64_t)slot_rows * (a.cache.head_dim + 2) * 4) / a.cache.kv_heads;
+}
 inline uint32_t split_target(const AttentionArgs& a, uint64_t wanted, uint64_t blocks, uint32_t slot_rows) {
-    const uint64_t units = most_units(a);
+    const uint64_t units = most_units(a), slots = split_slots(a, slot_rows);
     if (units >> 32 || blocks * units >> 31) return 1;
-    const uint64_t slots = a.part_bytes / ((uint64_t)slot_rows * (a.cache.head_dim + 2) * 4) / a.cache.kv_heads;
     const uint64_t most = slots > 2 * blocks ? slots - blocks : slots / 2;
     const uint64_t target = wanted < most ? wanted : most;
     return target < 1 ? 1 : (uint32_t)target;

@@ -402,7 +402,7 @@ hipError_t launch_tiles(const AttentionArgs& a, int cus) {
     // row blocks would not fit twice is left whole, which saves the join's launch.
     uint32_t target = split_target(a, 2ull * cus / kv, blocks, slot_rows);
     if (a.step.seqs == 1 && 2 * (whole + 1) > target) target = 1;
-    const Split split{target, ROWS, true};
+    const Split split{target, ROWS, (uint32_t)split_slots(a, slot_rows), true};
     attention_tiles_kernel<D><<<dim3(most_chunks(a, split.target, blocks) * kv), dim3(256), 0, a.stream>>>(a, split, slot_rows);
     return launch_join(a, split, blocks, slot_rows);
 }

@@ -635,6 +635,26 @@ def test_wrong_numbers_stay_inside_the_cache(mx4, ctx):
     near(from_bits(got[:10]), want[:10], tol[:10])
 
 
+def test_starts_that_do_not_ascend_end_well(mx4, ctx):
+    """Every second sequence claims all tokens, so that their work counts to 2^32: what comes of it is
+    nobody's, but nothing beside the outputs and the scratch is written, and later calls are right."""
+    rng = np.random.default_rng(31)
+    tokens, heads, d, page, seqs = 65536, 8, 64, 4096, 2048
+    side = np.full((3, 1, page, d), 0x3f80, np.uint16)
+    k, v = ctx.to_device(side), ctx.to_device(side)
+    start = ctx.to_device(np.array([0, tokens] * (seqs // 2) + [0], np.uint32))
+    cached, table = ctx.to_device(np.full(seqs, 65536, np.uint32)), ctx.to_device(rng.integers(0, 3, (seqs, 32)).astype(np.uint32))
+    q, out = ctx.to_device(to_bits(rng.standard_normal((tokens, heads * d)))), ctx.buffer(tokens * heads * d * 2)
+    after = ctx.to_device(np.full(1 << 20, 0x1234, np.uint16))
+    ctx.attention(q, heads, mx4.Batch(seqs, tokens, tokens, start, cached, table, 32), mx4.KvCache(k, v, 1, 3, 1, page, d), 0, out)
+    ctx.synchronize()
+    assert np.array_equal(k.download(np.uint16), side.ravel()) and np.array_equal(v.download(np.uint16), side.ravel())
+    assert np.all(after.download(np.uint16) == 0x1234)
+    step = Step(mx4, ctx, rng, [40, 1], [900, 3000], 2, 64, 16).fill(rng)
+    got, q = attend(step, rng, 8)
+    near(got, *reference(step, q, 8, chain(step)))
+
+
 def test_refusals(mx4, ctx):
     rng = np.random.default_rng(14)
     step = Step(mx4, ctx, rng, [2], [3], 2, 64, 16).fill(rng)
