@@ -6,7 +6,7 @@
 
 namespace mx4 {
 
-constexpr float kNoMax = -3.4028234664e38f;  // below every score: 2^(s - kNoMax) is never taken, -inf - kNoMax = -inf
+constexpr float kNoMax = -3.4028234664e38f;  // below every score; a masked one stays -inf less it
 // A row's maximum is raised only when a score passes it by this much: weights stay
 // below 2^8, their sums far inside f32, and most steps leave the accumulators alone.
 constexpr float kSlack = 8.0f;
