@@ -495,7 +495,7 @@ mx4_status mx4_qk_norm_rope(mx4_context *ctx, const mx4_qkv *in, const mx4_batch
  * (engine/src/gpu.metal:101-151; mx4_qk_norm_rope has put the new ones into the
  * cache): q_dev and out_dev bf16 rows of q_heads * head_dim (strides in
  * elements, 0: packed; rows 16-byte aligned), q_heads a multiple of the cache's
- * kv_heads. tree_dev NULL: new token i of a sequence sees the cached tokens and
+ * kv_heads; tokens * q_heads and seqs * kv_heads below 2^31. tree_dev NULL: new token i of a sequence sees the cached tokens and
  * the new ones 0 .. i. Otherwise tree_dev [tokens][tree_words] are masks: token
  * t sees the cached tokens and the new token j of its sequence if bit j % 64 of
  * tree_dev[t * tree_words + j / 64] is set (its own bit included). A token that

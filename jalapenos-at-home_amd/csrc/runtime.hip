@@ -1552,6 +1552,9 @@ mx4_status mx4_attention(mx4_context* ctx, const uint16_t* q, uint64_t q_stride,
     if (st != MX4_OK) return st;
     if (q_heads == 0 || q_heads > 65535 || q_heads % cache->kv_heads != 0)
         return fail(MX4_ERR_SHAPE, "q_heads must be a multiple of the cache's %u heads, at most 65535", cache->kv_heads);
+    // (row numbers and the grid are counted in 32 bits)
+    if ((uint64_t)a.step.tokens * q_heads >> 31 || (uint64_t)a.step.seqs * cache->kv_heads >> 31)
+        return fail(MX4_ERR_TOO_LARGE, "at most 2^31 - 1 query rows, and sequences times heads of the cache");
     if (!row_stride(q_stride, (uint64_t)q_heads * cache->head_dim, 2, &a.q_stride) ||
         !row_stride(out_stride, (uint64_t)q_heads * cache->head_dim, 2, &a.out_stride))
         return fail(MX4_ERR_SHAPE, "a stride is shorter than its row, breaks its alignment or is past 2^32 elements");

@@ -703,6 +703,15 @@ def test_refusals(mx4, ctx):
     rope(b=batch(tokens=0, max_tokens=0))
 
 
+def test_more_rows_than_32_bits_count_are_refused(mx4, ctx):
+    """Refused from the sizes alone: nothing of this size is there, and nothing is launched."""
+    buf = ctx.to_device(np.zeros(1 << 18, np.uint32))
+    for tokens, seqs, heads, kv_heads in [(1 << 30, 1, 2, 1), (1 << 20, 1, 2048, 8), (4, 65535, 65535, 65535)]:
+        cache = mx4.KvCache(buf, buf, 1, 1, kv_heads, 16, 64)
+        with pytest.raises(mx4.Mx4Error, match="2\\^31"):
+            ctx.attention(buf, heads, mx4.Batch(seqs, tokens, 1, buf, buf, buf, 1), cache, 0, buf)
+
+
 def test_example_decodes_the_same_tokens_by_trees(mx4):
     import importlib.util
     from pathlib import Path
