@@ -377,6 +377,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void attention_tiles_kernel(
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): nothing of the first pass is on its way to the slots
         fill();
     }
+    // The last tiles' loads (of nothing) end before the LDS can be another workgroup's.
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
     if (careful) {
         lds_barrier();
         if (tid == 0) again = 0;
